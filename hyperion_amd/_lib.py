@@ -9,6 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhypmi.so")
 
 HYPMI_MAX_SEG = 4
+F32, F16, BF16, F64 = 0, 1, 2, 3  # element types of the grouped operators
 SIDE_ENROL = 0
 SIDE_TEST = 1
 
@@ -181,6 +182,29 @@ SIGNATURES = {
     "hypmi_score_hist": (ctypes.c_int, [c_void_p, i64, i64, i64, c_void_p, c_void_p, c_void_p, c_void_p,
                                         i64, ctypes.c_float, ctypes.c_float, ctypes.c_int, c_void_p,
                                         c_void_p, c_void_p]),
+    "hypmi_grouped_weights_bytes": (i64, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "hypmi_grouped_columns_bytes": (i64, [ctypes.c_int, ctypes.c_int]),
+    "hypmi_grouped_weights": (ctypes.c_int, [c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, c_void_p,
+                                             c_void_p, c_void_p]),
+    "hypmi_grouped_affine": (ctypes.c_int, [c_void_p, ctypes.c_int, i64, ctypes.c_int, c_void_p, c_void_p,
+                                            ctypes.c_int, ctypes.c_int, i64, i64, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, ctypes.c_int, ctypes.c_int, c_void_p, i64, c_void_p]),
+    "hypmi_grouped_score_rows": (ctypes.c_int, [ctypes.c_int]),
+    "hypmi_grouped_score_span": (ctypes.c_int, []),
+    "hypmi_grouped_score": (ctypes.c_int, [c_void_p, i64, c_void_p, i64, ctypes.c_int, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, ctypes.c_int, i64, c_void_p, c_void_p]),
+    "hypmi_grouped_gram_span": (ctypes.c_int, []),
+    "hypmi_grouped_gram_workspace_bytes": (i64, [i64, ctypes.c_int]),
+    "hypmi_grouped_gram_f64": (ctypes.c_int, [c_void_p, ctypes.c_int, i64, ctypes.c_int, c_void_p, c_void_p, c_void_p,
+                                              c_void_p, ctypes.c_int, i64, i64, c_void_p, c_void_p, c_void_p,
+                                              c_void_p, i64, c_void_p]),
+    "hypmi_q4_ksteps": (ctypes.c_int, [ctypes.c_int]),
+    "hypmi_q4_task_rows": (ctypes.c_int, []),
+    "hypmi_q4_rows": (ctypes.c_int, [c_void_p, i64, ctypes.c_int, c_void_p, c_void_p, ctypes.c_int, i64, c_void_p,
+                                     c_void_p, c_void_p, c_void_p]),
+    "hypmi_q4_score": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int, c_void_p, i64, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, i64, c_void_p,
+                                      c_void_p]),
 }
 
 _lib = None

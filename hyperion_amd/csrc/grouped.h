@@ -1,0 +1,52 @@
+// Shared device code of the grouped operators (grouped_affine.hip, grouped_score.hip, grouped_gram.hip,
+// gallery.hip): rows that fall into groups of unequal sizes, delimited by offsets, are cut into tiles that
+// never cross a group; a workgroup finds its (group, tile) from a prefix sum of the tile counts.
+#pragma once
+#include "common.h"
+
+namespace hypmi_detail {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+// rows of caller arrays start at any multiple of their element size
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Largest e with prefix[e] <= t, for prefix[0] = 0 <= t < prefix[n]: the group of tile t (groups without
+// tiles share their successor's entry and are never returned).  All 64 lanes of a wave probe at once, so a
+// thousand groups take two dependent loads.  Call it with the whole wave active.
+__device__ __forceinline__ int find_group(const int64_t* __restrict__ prefix, int n, int64_t t) {
+    const int lane = (int)(threadIdx.x & 63);
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) >> 6;
+        const int64_t p = lo + (int64_t)(lane + 1) * step;
+        const bool le = p < hi && prefix[p] <= t;
+        const int c = __popcll(__ballot(le));
+        lo += c * step;
+        hi = lo + step < hi ? lo + step : hi;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Workgroups are handed to the eight XCDs round robin (a placement assumed for speed only); launch slot b
+// takes entry b / 8 of the eighth that belongs to its XCD, so that neighbouring tiles -- which read the same
+// group's operands -- meet in one L2.  Returns -1 for the slots that pad the grid.
+__device__ __forceinline__ int64_t xcd_slot(int64_t b, int64_t n) {
+    const int64_t per = (n + 7) >> 3;
+    const int64_t t = (b & 7) * per + (b >> 3);
+    return (b >> 3) < per && t < n ? t : -1;
+}
+
+inline int64_t xcd_grid(int64_t n) { return (n + 7) / 8 * 8; }
+
+// 2^e as a float, -126 <= e <= 127
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// x -> x0 + x1 with x0 = fp16(x), x1 = fp16(x - x0), four values: |x - x0 - x1| <= 2^-22 |x| while x1 is a
+// normal fp16 number.  An infinity becomes (inf, NaN): its products are NaN.
+__device__ __forceinline__ void split_pair4(f32x4 x, f16x4& x0, f16x4& x1) {
+    x0 = __builtin_convertvector(x, f16x4);
+    x1 = __builtin_convertvector(x - __builtin_convertvector(x0, f32x4), f16x4);
+}
+
+}  // namespace hypmi_detail

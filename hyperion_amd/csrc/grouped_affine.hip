@@ -1,0 +1,439 @@
+// Grouped affine map  y_r = x_r W_e + b_e  for every row r of group e, with an optional length
+// normalisation  y_r <- sqrt(dim_e) y_r / (|y_r| + 1e-10)  in the epilogue: one pre-processing or
+// projection matrix per recording, domain or speaker group (a chain step of
+// hyperion/transforms/cent_whiten.py:25-33, lda.py:31-34, pca.py:39-42, lnorm.py:14-17 whose parameters
+// depend on the row's group).
+//
+// Arithmetic.  Both operands are written as sums of two fp16 numbers, x = 2^-u (x0 + x1) with one power of
+// two per row, w = 2^-v (w0 + w1) with one per output column, and
+//     x w ~= 2^-(u + v) (x0 w0 + x0 w1 + x1 w0)
+// is accumulated in fp32 by v_mfma_f32_16x16x32_f16: the dropped product is 2^-22 |x w|, and a sum over d
+// coordinates has d / 32 times three roundings instead of d.  Vectors that come as fp16 or bf16 are exact in
+// x0 and take two products.  Against fp32 matrix instructions this is a third to a half of the issue time
+// of the same product.
+//
+// A row's scale has to be known before its first value is written, and the row is read once: the scale is
+// taken from the chunk of coordinates at hand (largest magnitude to [2^8, 2^9)), kept while later chunks stay
+// below 2^15, and lowered otherwise, with the sums so far multiplied by the (exact) power of two.  Six
+// powers of two of headroom cost nothing: x1 keeps 2^-33 of the row's largest magnitude.
+#include "grouped.h"
+
+namespace hypmi_detail {
+
+// four coordinates of a row as floats
+template <typename XT>
+struct Load4;
+template <>
+struct Load4<float> {
+    static __device__ __forceinline__ f32x4 get(const float* p) { return *reinterpret_cast<const f32x4_a4*>(p); }
+};
+typedef unsigned short u16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+template <>
+struct Load4<_Float16> {
+    static __device__ __forceinline__ f32x4 get(const _Float16* p) {
+        const u16x4_a2 r = *reinterpret_cast<const u16x4_a2*>(p);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)r[e]);
+        return v;
+    }
+};
+template <>
+struct Load4<__bf16> {
+    static __device__ __forceinline__ f32x4 get(const __bf16* p) {
+        const u16x4_a2 r = *reinterpret_cast<const u16x4_a2*>(p);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float((unsigned)r[e] << 16);
+        return v;
+    }
+};
+
+struct AffineArgs {
+    const void* x;
+    int64_t ldx;
+    int d_in;
+    const int64_t* offsets;  // [n_groups + 1]
+    const int64_t* tiles;    // [n_groups + 1] prefix of ceil(size / (16 RT))
+    int n_groups;
+    int64_t n_tiles;
+    const int32_t* order;    // row numbers grouped, or NULL
+    const uint4* w;          // fragments, see grouped_weights_kernel
+    const float* col;        // [n_groups][2][16 ct]: exponent of the inverse column scale (int), bias
+    const int32_t* dims;     // [n_groups] or NULL
+    int ct, ks, d_out;
+    float* y;
+    int64_t ldy;
+    int cols_y;              // columns written: d_out rounded up to four
+    int lnorm;
+};
+
+// RT row tiles of 16 per workgroup.  Eight waves: RS of them side by side along the rows, 8 / RS along the
+// output columns, two column tiles of 16 each.  Coordinates are taken in chunks of 512 / RT, so that every
+// thread holds sixteen values of a chunk whatever RT is; the chunk at hand sits in LDS as pairs in operand
+// order (lane l of a 16 x 32 tile: row l & 15, coordinates 8 (l >> 4) .. + 7; the row is XORed with
+// 4 (l >> 4) so that the four coordinate groups of a row fall into different banks when they are written),
+// the next one is on its way in registers.
+template <typename XT, int RT, int RS>
+__global__ __launch_bounds__(512) void grouped_affine_kernel(AffineArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int TM = 16 * RT;
+    constexpr int KC = 512 / RT;
+    constexpr int NP = sizeof(XT) == 4 ? 2 : 1;  // parts of x
+    constexpr int LPR = RT == 1 ? 32 : 16;       // lanes that load one row
+    constexpr int RPT = RT == 1 ? 1 : RT / 2;    // rows per thread
+    constexpr int F4 = 4 / RPT;                  // groups of four coordinates per thread and row
+    constexpr int CW = 8 / RS, RW = RT / RS, NT = 2;
+    constexpr int KSC = KC / 32;                 // k-steps per chunk
+    __shared__ uint4 tile[2][KSC * RT * NP * 64];
+    __shared__ int exps[2][TM];
+    __shared__ int64_t rows[TM];
+    __shared__ float norm[CW][TM];
+
+    const int64_t t = xcd_slot(blockIdx.x, g.n_tiles);
+    if (t < 0) return;
+    const int e = find_group(g.tiles, g.n_groups, t);
+    const int64_t r0 = g.offsets[e] + (t - g.tiles[e]) * TM;
+    const int64_t left = g.offsets[e + 1] - r0;
+    const int nrows = left < TM ? (int)left : TM;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < TM) {
+        const int64_t r = r0 + (tid < nrows ? tid : 0);
+        rows[tid] = g.order ? (int64_t)g.order[r] : r;
+    }
+    __syncthreads();
+
+    // ---- loading side: this thread's rows and coordinates
+    const int c = tid % LPR, rg = tid / LPR;
+    const XT* src[RPT];
+    int run[RPT];
+    f32x4 v[RPT][F4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        src[i] = static_cast<const XT*>(g.x) + rows[rg + (512 / LPR) * i] * g.ldx;
+        run[i] = 126;
+    }
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+            for (int f = 0; f < F4; ++f) {
+                const int k = k0 + 4 * (c + LPR * f);
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+                if (k + 4 <= g.d_in) {
+                    a = Load4<XT>::get(src[i] + k);
+                } else if (k < g.d_in) {
+                    for (int q = 0; q < g.d_in - k; ++q) a[q] = (float)src[i][k + q];
+                }
+                v[i][f] = a;
+            }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            float m = 0.f;
+#pragma unroll
+            for (int f = 0; f < F4; ++f)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(v[i][f][q]));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            const int ex = __builtin_amdgcn_frexp_expf(m);
+            if (m > 0.f && ex + run[i] > 15) run[i] = 9 - ex;
+            const float up = exp2_int(run[i]);
+            const int row = rg + (512 / LPR) * i;
+            if (c == 0) exps[buf][row] = run[i];
+            const int rt = row >> 4, r16 = row & 15;
+#pragma unroll
+            for (int f = 0; f < F4; ++f) {
+                const int k = 4 * (c + LPR * f);  // inside the chunk
+                const int s = k >> 5, kq = (k >> 3) & 3, half = (k >> 2) & 1;
+                f16x4 x0, x1;
+                split_pair4(v[i][f] * up, x0, x1);
+                f16x4* dst = reinterpret_cast<f16x4*>(
+                                 &tile[buf][((s * RT + rt) * NP) * 64 + kq * 16 + (r16 ^ (4 * kq))]) + half;
+                dst[0] = x0;
+                if (NP == 2) dst[2 * 64] = x1;
+            }
+        }
+    };
+
+    // ---- computing side
+    const int r16 = lane & 15, kq = lane >> 4;
+    const int wr = wave / CW, wc = wave % CW;
+    const int xs = kq * 16 + (r16 ^ (4 * kq));
+    int ctile[NT];
+    bool live[NT];
+    const uint4* wp[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        ctile[j] = (int)blockIdx.y * (CW * NT) + wc + CW * j;
+        live[j] = ctile[j] < g.ct;
+        wp[j] = g.w + (((int64_t)e * g.ct + (live[j] ? ctile[j] : 0)) * g.ks) * 128 + lane;
+    }
+    f32x4 acc[RW][NT];
+    int cur[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        cur[i] = 126;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int chunks = (g.d_in + KC - 1) / KC;
+    fetch(0);
+    store(0);
+    __syncthreads();
+    for (int ch = 0; ch < chunks; ++ch) {
+        const int buf = ch & 1;
+        if (ch + 1 < chunks) fetch((ch + 1) * KC);
+        if (live[0]) {
+            bool moved = false;
+            int now[RW];
+#pragma unroll
+            for (int i = 0; i < RW; ++i) {
+                now[i] = exps[buf][16 * (wr * RW + i) + r16];
+                moved |= now[i] != cur[i];
+            }
+            if (__any(moved)) {
+#pragma unroll
+                for (int i = 0; i < RW; ++i) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[i][j][q] = ldexpf(acc[i][j][q], now[i] - cur[i]);
+                    cur[i] = now[i];
+                }
+            }
+            const int smax = g.ks - ch * KSC < KSC ? g.ks - ch * KSC : KSC;
+            for (int s = 0; s < smax; ++s) {
+                f16x8 w0[NT], w1[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint4* p = wp[j] + (int64_t)(ch * KSC + s) * 128;
+                    w0[j] = __builtin_bit_cast(f16x8, p[0]);
+                    w1[j] = __builtin_bit_cast(f16x8, p[64]);
+                }
+#pragma unroll
+                for (int i = 0; i < RW; ++i) {
+                    const uint4* xp = &tile[buf][((s * RT + wr * RW + i) * NP) * 64 + xs];
+                    const f16x8 x0 = __builtin_bit_cast(f16x8, xp[0]);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w1[j], x0, acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0[j], x0, acc[i][j], 0, 0, 0);
+                    }
+                    if constexpr (NP == 2) {
+                        const f16x8 x1 = __builtin_bit_cast(f16x8, xp[64]);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0[j], x1, acc[i][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (ch + 1 < chunks) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    // ---- epilogue: lane holds columns 16 ctile + 4 kq .. + 3 of row 16 (wr RW + i) + r16
+    const int cp = 16 * g.ct;
+    const float* col = g.col + (int64_t)e * 2 * cp;
+    float ss[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) ss[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        if (!live[j]) continue;
+        const int4 sc = *reinterpret_cast<const int4*>(col + 16 * ctile[j] + 4 * kq);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(col + cp + 16 * ctile[j] + 4 * kq);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            // one shift by the sum of both exponents: neither scale alone may leave the range
+            acc[i][j][0] = ldexpf(acc[i][j][0], sc.x - cur[i]) + b[0];
+            acc[i][j][1] = ldexpf(acc[i][j][1], sc.y - cur[i]) + b[1];
+            acc[i][j][2] = ldexpf(acc[i][j][2], sc.z - cur[i]) + b[2];
+            acc[i][j][3] = ldexpf(acc[i][j][3], sc.w - cur[i]) + b[3];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) ss[i] = fmaf(acc[i][j][q], acc[i][j][q], ss[i]);
+        }
+    }
+    float factor[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) factor[i] = 1.f;
+    if (g.lnorm) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            ss[i] += __shfl_xor(ss[i], 16);
+            ss[i] += __shfl_xor(ss[i], 32);
+            if (kq == 0) norm[wc][16 * (wr * RW + i) + r16] = ss[i];
+        }
+        __syncthreads();
+        const float top = sqrtf((float)(g.dims ? g.dims[e] : g.d_out));
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < CW; ++w) s += norm[w][16 * (wr * RW + i) + r16];
+            factor[i] = top / (sqrtf(s) + 1e-10f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int row = 16 * (wr * RW + i) + r16;
+        if (row >= nrows) continue;
+        float* out = g.y + rows[row] * g.ldy;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int c0 = 16 * ctile[j] + 4 * kq;
+            if (live[j] && c0 < g.cols_y) *reinterpret_cast<f32x4*>(out + c0) = acc[i][j] * factor[i];
+        }
+    }
+#endif
+}
+
+// W [n_groups][d_in][d_out] -> operand fragments w[n_groups][ct][ks][part][lane] (16 bytes each: column
+// 16 ct + (lane & 15), coordinates 32 ks + 8 (lane >> 4) .. + 7, zero outside W) and col[n_groups][2][16 ct]
+// (exponent of the inverse scale as an int, bias).  One workgroup per (group, column tile).
+__global__ __launch_bounds__(256) void grouped_weights_kernel(const float* __restrict__ W, const float* __restrict__ b,
+                                                              int d_in, int d_out, int ct, int ks,
+                                                              uint4* __restrict__ w, float* __restrict__ col) {
+    __shared__ float top[16][17];
+    const int64_t e = blockIdx.x / ct;
+    const int j = (int)(blockIdx.x - e * ct);
+    const int c = threadIdx.x & 15, kg = threadIdx.x >> 4;
+    const int cc = 16 * j + c;
+    const float* src = W + (e * d_in) * d_out + cc;
+    float m = 0.f;
+    if (cc < d_out)
+        for (int k = kg; k < d_in; k += 16) {
+            const float a = fabsf(src[(int64_t)k * d_out]);
+            if (a <= 3.402823466e38f) m = fmaxf(m, a);
+        }
+    top[kg][c] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, top[i][c]);
+    int up = m > 0.f ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
+    if (kg == 0) {
+        float* dst = col + e * 32 * ct;
+        dst[cc] = __int_as_float(-up);
+        dst[16 * ct + cc] = (b && cc < d_out) ? b[e * d_out + cc] : 0.f;
+    }
+    uint4* out = w + ((e * ct + j) * ks) * 128;
+    for (int kb = kg; kb < 4 * ks; kb += 16) {  // blocks of eight coordinates
+        f16x8 p0, p1;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int k = 8 * kb + q;
+            const float x = (cc < d_out && k < d_in) ? ldexpf(src[(int64_t)k * d_out], up) : 0.f;
+            p0[q] = (_Float16)x;
+            p1[q] = (_Float16)(x - (float)p0[q]);
+        }
+        uint4* dst = out + (kb >> 2) * 128 + (kb & 3) * 16 + c;
+        dst[0] = __builtin_bit_cast(uint4, p0);
+        dst[64] = __builtin_bit_cast(uint4, p1);
+    }
+}
+
+// Length normalisation of rows of y by group where a row does not fit one workgroup of the product
+// (more than 256 output columns): one wave per listed row.
+__global__ __launch_bounds__(256) void grouped_lnorm_kernel(float* __restrict__ y, int64_t ldy, int d_out,
+                                                            const int64_t* __restrict__ offsets, int n_groups,
+                                                            const int32_t* __restrict__ order,
+                                                            const int32_t* __restrict__ dims, int64_t n) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= n) return;
+    const int lane = threadIdx.x & 63;
+    float top = (float)d_out;
+    if (dims) top = (float)dims[find_group(offsets, n_groups, r)];
+    float* row = y + (order ? (int64_t)order[r] : r) * ldy;
+    float s = 0.f;
+    for (int k = lane; k < d_out; k += 64) s = fmaf(row[k], row[k], s);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    const float f = sqrtf(top) / (sqrtf(s) + 1e-10f);
+    for (int k = lane; k < d_out; k += 64) row[k] *= f;
+}
+
+template <typename XT, int RT, int RS>
+int launch_affine(const AffineArgs& g, hipStream_t stream) {
+    const int per = 2 * (8 / RS);
+    const int64_t gx = xcd_grid(g.n_tiles), gy = (g.ct + per - 1) / per;
+    HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
+    hipLaunchKernelGGL((grouped_affine_kernel<XT, RT, RS>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, stream, g);
+    HYPMI_HIP(hipGetLastError());
+    return HYPMI_OK;
+}
+
+template <typename XT>
+int launch_affine_type(const AffineArgs& g, int tile_rows, hipStream_t stream) {
+    switch (tile_rows) {
+        case 16: return launch_affine<XT, 1, 1>(g, stream);
+        case 64: return launch_affine<XT, 4, 1>(g, stream);
+        default: return launch_affine<XT, 8, 1>(g, stream);
+    }
+}
+
+}  // namespace hypmi_detail
+
+using namespace hypmi_detail;
+
+extern "C" int64_t hypmi_grouped_weights_bytes(int n_groups, int d_in, int d_out) {
+    if (n_groups < 0 || d_in <= 0 || d_out <= 0) return 0;
+    return (int64_t)n_groups * ((d_out + 15) / 16) * ((d_in + 31) / 32) * 2048;
+}
+
+extern "C" int64_t hypmi_grouped_columns_bytes(int n_groups, int d_out) {
+    if (n_groups < 0 || d_out <= 0) return 0;
+    return (int64_t)n_groups * 2 * ((d_out + 15) / 16 * 16) * 4;
+}
+
+extern "C" int hypmi_grouped_weights(const float* W, const float* b, int n_groups, int d_in, int d_out, void* w,
+                                     void* columns, void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    HYPMI_REQUIRE(n_groups >= 0 && d_in > 0 && d_out > 0, "grouped_weights: bad shape");
+    if (n_groups == 0) return HYPMI_OK;
+    HYPMI_REQUIRE(W && w && columns, "grouped_weights: null pointer");
+    HYPMI_REQUIRE(aligned16(w) && aligned16(columns), "grouped_weights: buffers must be 16-byte aligned");
+    const int ct = (d_out + 15) / 16, ks = (d_in + 31) / 32;
+    const int64_t blocks = (int64_t)n_groups * ct;
+    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_weights: too many groups");
+    hipLaunchKernelGGL(grouped_weights_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, W, b, d_in, d_out, ct, ks,
+                       static_cast<uint4*>(w), static_cast<float*>(columns));
+    HYPMI_HIP(hipGetLastError());
+    return HYPMI_OK;
+}
+
+extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int d_in, const int64_t* offsets,
+                                    const int64_t* tiles, int tile_rows, int n_groups, int64_t n_rows,
+                                    int64_t n_tiles, const int32_t* order, const void* w, const void* columns,
+                                    const int32_t* dims, int d_out, int lnorm, float* y, int64_t ldy, void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    HYPMI_REQUIRE(n_groups >= 0 && n_rows >= 0 && n_tiles >= 0 && d_in > 0 && d_out > 0, "grouped_affine: bad shape");
+    HYPMI_REQUIRE(x_type >= HYPMI_F32 && x_type <= HYPMI_BF16, "grouped_affine: vectors must be fp32, fp16 or bf16");
+    HYPMI_REQUIRE(tile_rows == 16 || tile_rows == 64 || tile_rows == 128, "grouped_affine: tiles of 16, 64 or 128 rows");
+    const int cols_y = (d_out + 3) / 4 * 4;
+    HYPMI_REQUIRE(ldx >= d_in && ldy >= cols_y && ldy % 4 == 0, "grouped_affine: bad leading dimension");
+    if (n_tiles == 0) return HYPMI_OK;
+    HYPMI_REQUIRE(x && offsets && tiles && w && columns && y, "grouped_affine: null pointer");
+    HYPMI_REQUIRE(aligned16(w) && aligned16(columns) && aligned16(y), "grouped_affine: buffers must be 16-byte aligned");
+    const int ct = (d_out + 15) / 16;
+    const bool fused = lnorm && ct <= 16;
+    AffineArgs g = {x, ldx, d_in, offsets, tiles, n_groups, n_tiles, order, static_cast<const uint4*>(w),
+                    static_cast<const float*>(columns), dims, ct, (d_in + 31) / 32, d_out, y, ldy, cols_y, fused};
+    int rc;
+    switch (x_type) {
+        case HYPMI_F32: rc = launch_affine_type<float>(g, tile_rows, stream); break;
+        case HYPMI_F16: rc = launch_affine_type<_Float16>(g, tile_rows, stream); break;
+        default: rc = launch_affine_type<__bf16>(g, tile_rows, stream); break;
+    }
+    if (rc != HYPMI_OK || !lnorm || fused) return rc;
+    const int64_t blocks = (n_rows + 3) / 4;
+    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_affine: too many rows");
+    hipLaunchKernelGGL(grouped_lnorm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, y, ldy, d_out, offsets,
+                       n_groups, order, dims, n_rows);
+    HYPMI_HIP(hipGetLastError());
+    return HYPMI_OK;
+}

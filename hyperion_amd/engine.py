@@ -612,3 +612,7 @@ def to_host(t, dtype):
     pending[2].synchronize()
     dst[pending[1][0]:pending[1][1]].copy_(pending[0])
     return out
+
+
+from .grouped import (AffineBank, GroupPairs, Q4Rows, RowGroups, grouped_affine, grouped_gram64,  # noqa: E402,F401
+                      grouped_score, q4_rows, q4_score)

@@ -1,0 +1,437 @@
+"""Grouped operators: rows that fall into groups of unequal sizes (the recordings of a batch, the domains
+of a trial set, the partitions of a gallery), each group with its own matrix, its own moments or its own
+block of scores, in one launch.  The names here are part of hyperion_amd.engine.
+
+A batch is described once, by a RowGroups (sizes on the host, tables on the device) and, for products of
+two sides, a GroupPairs; the operators themselves neither wait for the device nor send it anything, so they
+can be captured in a HIP graph.  Inputs have to be on one device; the work runs on that device's current
+stream."""
+import numpy as np
+
+from . import _lib, engine
+from .engine import _ptr, _torch, round_up
+
+_AFFINE_TILES = (16, 64, 128)
+
+
+def _prefix(counts):
+    out = np.zeros(len(counts) + 1, dtype=np.int64)
+    np.cumsum(counts, out=out[1:])
+    return out
+
+
+def _ceil(a, b):
+    return -(-a // b)
+
+
+def _device(device=None):
+    torch = engine.require_gpu()
+    d = torch.device("cuda" if device is None else device)
+    if d.type != "cuda":
+        raise ValueError("the grouped operators work on the GPU, not on %s" % d)
+    return torch.device("cuda", torch.cuda.current_device() if d.index is None else d.index)
+
+
+def _tables(arrays, device):
+    """Host int64 tables of equal length as rows of one device tensor (one copy, complete on return)."""
+    torch = _torch()
+    return torch.from_numpy(np.ascontiguousarray(np.stack(arrays))).to(device)
+
+
+def _keep(stream, *tensors):
+    """Storage that outlives its last Python reference until `stream` has used it."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
+class RowGroups:
+    """Rows in groups: group e owns `sizes[e]` consecutive rows (zero is allowed), in order, or, with
+    `order`, the rows order[offsets[e]] .. order[offsets[e + 1] - 1]; every row may be listed once.
+    sizes: host integers.  order: host or device integers, one per listed row."""
+
+    def __init__(self, sizes, order=None, device=None):
+        sizes = np.asarray(sizes)
+        if sizes.ndim != 1 or (sizes.size and sizes.dtype.kind not in "iu"):
+            raise ValueError("group sizes must be a 1-D sequence of integers")
+        sizes = sizes.astype(np.int64)
+        if sizes.size and sizes.min() < 0:
+            raise ValueError("group sizes must not be negative")
+        if sizes.size > 0x7fffffff:
+            raise ValueError("at most 2^31 - 1 groups")
+        self.sizes = sizes
+        self.offsets = _prefix(sizes)
+        self.num_groups = int(sizes.size)
+        self.total = int(self.offsets[-1])
+        self.device = _device(device)
+        self.order = None
+        self.num_rows = self.total  # rows an input needs at least
+        if order is not None:
+            self._set_order(order)
+        lib = _lib.load()
+        span = lib.hypmi_grouped_gram_span()
+        cut = _ceil(sizes, span)
+        prefix = [_prefix(_ceil(sizes, t)) for t in _AFFINE_TILES]
+        chunks, slots = _prefix(np.maximum(cut, 1)), _prefix(np.where(cut > 1, cut, 0))
+        self._tab = _tables([self.offsets] + prefix + [chunks, slots], self.device)
+        self._n_tiles = dict(zip(_AFFINE_TILES, (int(p[-1]) for p in prefix)))
+        self._n_chunks, self._n_slots = int(chunks[-1]), int(slots[-1])
+
+    @classmethod
+    def from_ids(cls, ids, num_groups=None, device=None):
+        """Groups of rows by a group number per row, 0 .. num_groups - 1 (default: the largest + 1)."""
+        ids = np.asarray(ids)
+        if ids.ndim != 1 or (ids.size and ids.dtype.kind not in "iu"):
+            raise ValueError("group ids must be a 1-D sequence of integers")
+        ids = ids.astype(np.int64)
+        top = int(ids.max()) + 1 if ids.size else 0
+        if num_groups is None:
+            num_groups = top
+        if ids.size and (ids.min() < 0 or top > num_groups):
+            raise ValueError("group ids must lie in 0 .. %d" % (num_groups - 1))
+        return cls(np.bincount(ids, minlength=num_groups), np.argsort(ids, kind="stable"), device)
+
+    def _set_order(self, order):
+        torch = _torch()
+        if not isinstance(order, torch.Tensor):
+            order = torch.from_numpy(np.ascontiguousarray(order))
+        if order.dim() != 1 or order.dtype not in (torch.int32, torch.int64):
+            raise ValueError("order must be a 1-D sequence of integers")
+        if order.numel() != self.total:
+            raise ValueError("order lists %d rows, the groups hold %d" % (order.numel(), self.total))
+        if self.total:
+            lo, hi = int(order.min()), int(order.max())
+            if lo < 0 or hi > 0x7fffffff:
+                raise ValueError("order must hold row numbers from 0 to 2^31 - 1")
+            self.num_rows = hi + 1
+            order = order.to(self.device)
+            seen = torch.zeros(hi + 1, dtype=torch.int8, device=self.device)
+            seen[order.long()] = 1
+            if int(seen.sum(dtype=torch.int64)) != self.total:
+                raise ValueError("order lists a row more than once")
+        self.order = order.to(device=self.device, dtype=torch.int32).contiguous()
+
+    def _row(self, i):
+        """Device pointer of table row i: 0 offsets, 1 .. 3 tile prefixes, 4 chunks, 5 slots."""
+        return self._tab.data_ptr() + 8 * i * (self.num_groups + 1)
+
+    def _check(self, x, what):
+        if x.device != self.device:
+            raise ValueError("%s is on %s, its groups are on %s" % (what, x.device, self.device))
+        if self.order is None:
+            if x.shape[0] != self.total:
+                raise ValueError("%s has %d rows, its groups hold %d" % (what, x.shape[0], self.total))
+        elif x.shape[0] < self.num_rows:
+            raise ValueError("%s has %d rows, the order names row %d" % (what, x.shape[0], self.num_rows - 1))
+
+
+class GroupPairs:
+    """Blocks of scores of two sides that have the same groups: block e is rows.sizes[e] x cols.sizes[e],
+    the blocks lie one after the other in a flat result without padding."""
+
+    def __init__(self, rows, cols):
+        if rows.num_groups != cols.num_groups:
+            raise ValueError("the two sides have %d and %d groups" % (rows.num_groups, cols.num_groups))
+        if rows.device != cols.device:
+            raise ValueError("the two sides are on %s and %s" % (rows.device, cols.device))
+        if rows.order is not None or cols.order is not None:
+            raise ValueError("score blocks need rows in group order (RowGroups without order)")
+        self.rows, self.cols = rows, cols
+        self.device = rows.device
+        n1, n2 = rows.sizes, cols.sizes
+        self.offsets = _prefix(n1 * n2)
+        self.numel = int(self.offsets[-1])
+        lib = _lib.load()
+        span, run = lib.hypmi_grouped_score_span(), lib.hypmi_q4_task_rows()
+        top = int(n1.max()) if n1.size else 0
+        self._q4_tests = 16 if top <= 16 else 32 if top <= 32 else 64
+        tabs = [_prefix(_ceil(n1, b) * _ceil(n2, span)) for b in (64, 128)]
+        tabs.append(_prefix(_ceil(n1, self._q4_tests) * _ceil(n2, run)))
+        self._n_tasks = [int(t[-1]) for t in tabs]
+        self._tab = _tables([self.offsets] + tabs, self.device)
+
+    def _row(self, i):
+        """Device pointer of table row i: 0 block offsets, 1 and 2 score tasks (64 and 128 rows), 3 gallery tasks."""
+        return self._tab.data_ptr() + 8 * i * (self.rows.num_groups + 1)
+
+    def block(self, flat, e):
+        """Block e of a flat result as a [rows, cols] view."""
+        return flat[int(self.offsets[e]):int(self.offsets[e + 1])].view(int(self.rows.sizes[e]), int(self.cols.sizes[e]))
+
+    def blocks(self, flat):
+        return [self.block(flat, e) for e in range(self.rows.num_groups)]
+
+    def _result(self, out):
+        torch = _torch()
+        if out is None:
+            return torch.empty(self.numel, dtype=torch.float32, device=self.device)
+        if out.dtype != torch.float32 or out.device != self.device or out.dim() != 1 or out.numel() != self.numel \
+                or not out.is_contiguous():
+            raise ValueError("out must be a contiguous fp32 vector of %d elements on %s" % (self.numel, self.device))
+        return out
+
+
+class AffineBank:
+    """One affine map per group, x -> x W[e] + b[e], laid out for grouped_affine.  W [E, d_in, d_out] and b
+    [E, d_out] (or None), host arrays or device tensors of any float type, kept at fp32 accuracy.  dims
+    [E] (optional): dimension of every map where they differ; W[e][:, dims[e]:] and b[e][dims[e]:] have to be
+    zero, and the length normalisation scales to sqrt(dims[e])."""
+
+    def __init__(self, W, b=None, dims=None, device=None):
+        torch = _torch()
+        if device is None and isinstance(W, torch.Tensor) and W.is_cuda:
+            device = W.device
+        self.device = _device(device)
+        W = self._fp32(W)
+        if W.dim() != 3 or 0 in W.shape[1:]:
+            raise ValueError("W must be [groups, d_in, d_out], got %s" % (tuple(W.shape),))
+        self.num_groups, self.d_in, self.d_out = (int(v) for v in W.shape)
+        if b is not None:
+            b = self._fp32(b)
+            if tuple(b.shape) != (self.num_groups, self.d_out):
+                raise ValueError("b must be [%d, %d], got %s" % (self.num_groups, self.d_out, tuple(b.shape)))
+        self.dims = None
+        if dims is not None:
+            dims = np.asarray(dims)
+            if dims.shape != (self.num_groups,) or dims.dtype.kind not in "iu" or \
+                    (dims.size and (dims.min() < 1 or dims.max() > self.d_out)):
+                raise ValueError("dims must be %d integers in 1 .. %d" % (self.num_groups, self.d_out))
+            self.dims = torch.from_numpy(dims.astype(np.int32)).to(self.device)
+        lib = _lib.load()
+        args = (self.num_groups, self.d_in, self.d_out)
+        self._w = torch.empty(lib.hypmi_grouped_weights_bytes(*args) // 4, dtype=torch.int32, device=self.device)
+        self._c = torch.empty(lib.hypmi_grouped_columns_bytes(self.num_groups, self.d_out) // 4, dtype=torch.float32,
+                              device=self.device)
+        if self.num_groups:
+            with torch.cuda.device(self.device):
+                _lib.check(lib.hypmi_grouped_weights(_ptr(W), None if b is None else _ptr(b), *args, _ptr(self._w),
+                                                     _ptr(self._c), engine.stream_ptr()))
+
+    def _fp32(self, a):
+        torch = _torch()
+        if not isinstance(a, torch.Tensor):
+            a = torch.from_numpy(np.ascontiguousarray(a))
+        if not a.is_floating_point():
+            raise ValueError("weights must be floating-point numbers")
+        return a.to(device=self.device, dtype=torch.float32).contiguous()
+
+
+def _device_rows(x, types, what):
+    """A 2-D device tensor of one of `types` with unit column stride, as it is; a view with other strides is
+    copied.  Returns (x, leading dimension)."""
+    torch = engine.require_gpu()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("%s must be a device tensor" % what)
+    if x.dim() != 2:
+        raise ValueError("%s must be 2-D, got shape %s" % (what, tuple(x.shape)))
+    if x.dtype not in types:
+        raise ValueError("%s is %s, expected one of %s" % (what, x.dtype, ", ".join(str(t) for t in types)))
+    n, d = x.shape
+    if (d > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < d):
+        x = x.contiguous()
+    return x, (x.stride(0) if n > 1 else d)
+
+
+def grouped_affine(x, groups, bank, lnorm=False, out=None):
+    """y_r = x_r W_e + b_e for every row r of group e, with lnorm followed by the length normalisation
+    y <- sqrt(dim_e) y / (|y| + 1e-10).  x: device fp32, fp16 or bf16 [n, d_in]; returns device fp32
+    [n, d_out] (fp32 accuracy).  With an ordered RowGroups row i of the result belongs to row i of x; rows of
+    no group are zero in a new result and left alone in `out` (fp32, 16-byte aligned rows)."""
+    torch = engine.require_gpu()
+    kinds = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+    x, ldx = _device_rows(x, kinds, "x")
+    groups._check(x, "x")
+    if bank.device != groups.device:
+        raise ValueError("the maps are on %s, the groups on %s" % (bank.device, groups.device))
+    if bank.num_groups != groups.num_groups:
+        raise ValueError("%d maps for %d groups" % (bank.num_groups, groups.num_groups))
+    if x.shape[1] != bank.d_in:
+        raise ValueError("expected %d-dim vectors, got %d" % (bank.d_in, x.shape[1]))
+    n, d = x.shape[0], bank.d_out
+    ld = round_up(d, 4)
+    if out is None:
+        make = torch.empty if groups.total == n else torch.zeros
+        y = make((n, ld), dtype=torch.float32, device=x.device)
+    else:
+        y = out
+        if y.dtype != torch.float32 or y.device != x.device or tuple(y.shape) != (n, d) or \
+                (d > 1 and y.stride(1) != 1) or y.data_ptr() % 16 or (n > 1 and (y.stride(0) % 4 or y.stride(0) < ld)):
+            raise ValueError("out must be fp32 [%d, %d] on %s with 16-byte aligned rows of at least %d elements"
+                             % (n, d, x.device, ld))
+        if n and (y.untyped_storage().nbytes() // 4 - y.storage_offset()) < (n - 1) * y.stride(0) + ld:
+            raise ValueError("the last row of out has no room for %d elements" % ld)
+        if _overlap(x, y):
+            raise ValueError("out must not share memory with x")
+    tile = _affine_tile(groups)
+    n_tiles = groups._n_tiles[tile]
+    if n_tiles:
+        with torch.cuda.device(x.device):
+            stream = torch.cuda.current_stream()
+            _keep(stream, groups._tab, groups.order, bank._w, bank._c, bank.dims)
+            _lib.check(_lib.load().hypmi_grouped_affine(
+                _ptr(x), kinds[x.dtype], ldx, bank.d_in, groups._row(0), groups._row(1 + _AFFINE_TILES.index(tile)),
+                tile, groups.num_groups, groups.total, n_tiles, None if groups.order is None else _ptr(groups.order),
+                _ptr(bank._w), _ptr(bank._c), None if bank.dims is None else _ptr(bank.dims), d, int(bool(lnorm)),
+                _ptr(y), ld if out is None else (y.stride(0) if n > 1 else ld), engine.stream_ptr()))
+    return y[:, :d] if out is None else out
+
+
+def _affine_tile(groups):
+    """Rows per workgroup: the largest tile that most rows can fill."""
+    used = int(np.count_nonzero(groups.sizes))
+    mean = groups.total / used if used else 0
+    return 16 if mean <= 16 else 64 if mean <= 1000 else 128
+
+
+def _overlap(a, b):
+    """Whether the storage ranges of two tensors meet."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        lo = t.data_ptr()
+        return lo, lo + t.element_size() * (1 + sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())))
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _packed(G, groups, what):
+    """Packed rows as the grouped kernels take them: fp32, 16-byte aligned rows."""
+    torch = engine.require_gpu()
+    G, ld = _device_rows(G, (torch.float32,), what)
+    groups._check(G, what)
+    if G.data_ptr() % 16 or ld % 4:
+        raise ValueError("%s must have 16-byte aligned rows" % what)
+    return G, ld
+
+
+def grouped_score(G1, G2, pairs, out=None):
+    """Scores of packed enrol rows against packed test rows of the same group (Plan.prologue, both [n, kp]):
+    the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e)."""
+    G1, ld1 = _packed(G1, pairs.rows, "G1")
+    G2, ld2 = _packed(G2, pairs.cols, "G2")
+    kp = G1.shape[1]
+    if G2.shape[1] != kp:
+        raise ValueError("packed widths differ: %d vs %d" % (kp, G2.shape[1]))
+    lib = _lib.load()
+    rows = lib.hypmi_grouped_score_rows(kp)
+    if not rows:
+        raise ValueError("packed width %d has no grouped kernel (multiples of 8 up to 512)" % kp)
+    S = pairs._result(out)
+    i = 1 if rows == 64 else 2
+    if pairs.numel:
+        torch = _torch()
+        with torch.cuda.device(pairs.device):
+            _keep(torch.cuda.current_stream(), pairs._tab, pairs.rows._tab, pairs.cols._tab)
+            _lib.check(lib.hypmi_grouped_score(_ptr(G1), ld1, _ptr(G2), ld2, kp, pairs.rows._row(0), pairs.cols._row(0),
+                                               pairs._row(0), pairs._row(i), pairs.rows.num_groups,
+                                               pairs._n_tasks[i - 1], _ptr(S), engine.stream_ptr()))
+    return S
+
+
+def grouped_gram64(x, groups, w=None):
+    """(sum_r w_r x_r x_r^T, sum_r w_r x_r) of every group as device float64 tensors [E, d, d] and [E, d]; x
+    device fp32 or float64 [n, d], w optional float64 weights per row of x."""
+    torch = engine.require_gpu()
+    kinds = {torch.float32: _lib.F32, torch.float64: _lib.F64}
+    x, ldx = _device_rows(x, kinds, "x")
+    groups._check(x, "x")
+    d, E = x.shape[1], groups.num_groups
+    if d < 1:
+        raise ValueError("x has no columns")
+    if w is not None:
+        if not isinstance(w, torch.Tensor) or w.device != x.device or w.dtype != torch.float64 or \
+                tuple(w.shape) != (x.shape[0],):
+            raise ValueError("w must be a float64 vector of %d elements on %s" % (x.shape[0], x.device))
+        w = w.contiguous()
+    lib = _lib.load()
+    C = torch.empty((E, d, d), dtype=torch.float64, device=x.device)
+    F = torch.empty((E, d), dtype=torch.float64, device=x.device)
+    nbytes = lib.hypmi_grouped_gram_workspace_bytes(groups._n_slots, d)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
+    if E:
+        with torch.cuda.device(x.device):
+            _keep(torch.cuda.current_stream(), groups._tab, groups.order)
+            _lib.check(lib.hypmi_grouped_gram_f64(
+                _ptr(x), kinds[x.dtype], ldx, d, None if w is None else _ptr(w), groups._row(0), groups._row(4),
+                groups._row(5), E, groups._n_chunks, groups._n_slots,
+                None if groups.order is None else _ptr(groups.order), _ptr(C), _ptr(F),
+                None if ws is None else _ptr(ws), nbytes, engine.stream_ptr()))
+    return C, F
+
+
+class Q4Rows:
+    """Packed enrol-side rows held in 4 bits (q4_rows makes them)."""
+
+    def __init__(self, codes, scales, q, k, groups):
+        self.codes, self.scales, self.q, self.k, self.groups = codes, scales, q, k, groups
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.q))
+
+    def values(self):
+        """The coordinates that the codes stand for, device fp32 [n, k]."""
+        torch = _torch()
+        ks = self.codes.shape[1]
+        w = self.codes.view(-1, ks, 4, 16, 4)  # block, k-step, coordinates 8 i .. 8 i + 7, row & 15, row >> 4
+        shifts = torch.tensor([8 * (j >> 2) + 4 * ((j >> 1) & 1) + 16 * (j & 1) for j in range(8)],
+                              dtype=torch.int32, device=w.device)
+        c = (w[..., None] >> shifts & 15).float() - 8
+        s = (self.scales.view(-1, ks, 1, 16, 4, 1).to(torch.int32) << 16).view(torch.float32)
+        v = (c * s).permute(0, 4, 3, 1, 2, 5).reshape(-1, ks * 32)
+        g = self.groups
+        keep = np.concatenate([np.arange(n) + 64 * b for n, b in zip(g.sizes, _prefix(_ceil(g.sizes, 64)))]
+                              or [np.zeros(0)]).astype(np.int64)
+        return v[torch.from_numpy(keep).to(v.device)][:, :self.k].contiguous()
+
+
+def q4_rows(G, k, groups=None):
+    """Packed enrol-side rows [g, q, 1] (Plan.prologue; k coordinates) -> Q4Rows.  groups: partitions of the
+    gallery (default: one)."""
+    torch = engine.require_gpu()
+    G, ld = _device_rows(G, (torch.float32,), "G")
+    if groups is None:
+        groups = RowGroups([G.shape[0]], device=G.device)
+    groups._check(G, "G")
+    if groups.order is not None:
+        raise ValueError("a gallery needs rows in group order (RowGroups without order)")
+    lib = _lib.load()
+    ks = lib.hypmi_q4_ksteps(int(k))
+    if not ks or G.shape[1] < k + 1:
+        raise ValueError("%d coordinates in rows of %d (1 to 512 coordinates, then q)" % (k, G.shape[1]))
+    nb = groups._n_tiles[64]
+    codes = torch.empty((nb, ks, 64, 4), dtype=torch.int32, device=G.device)
+    scales = torch.empty((nb, ks, 16, 4), dtype=torch.int16, device=G.device)
+    q = torch.empty((nb, 64), dtype=torch.float32, device=G.device)
+    if nb:
+        with torch.cuda.device(G.device):
+            _keep(torch.cuda.current_stream(), groups._tab)
+            _lib.check(lib.hypmi_q4_rows(_ptr(G), ld, int(k), groups._row(0), groups._row(2), groups.num_groups, nb,
+                                         _ptr(codes), _ptr(scales), _ptr(q), engine.stream_ptr()))
+    return Q4Rows(codes, scales, q, int(k), groups)
+
+
+def q4_score(gallery, G, pairs, out=None):
+    """Scores of packed test-side rows [g, 1, q + c] against a 4-bit gallery, group by group: the flat device
+    fp32 result of `pairs` = GroupPairs(test groups, gallery.groups); block e is [tests, gallery rows]."""
+    torch = engine.require_gpu()
+    if pairs.cols is not gallery.groups and not np.array_equal(pairs.cols.sizes, gallery.groups.sizes):
+        raise ValueError("the columns of pairs are not the groups of the gallery")
+    G, ld = _device_rows(G, (torch.float32,), "G")
+    pairs.rows._check(G, "G")
+    if gallery.codes.device != pairs.device:
+        raise ValueError("the gallery is on %s, the groups on %s" % (gallery.codes.device, pairs.device))
+    if G.shape[1] < gallery.k + 2:
+        raise ValueError("packed rows of %d elements for a gallery of %d coordinates" % (G.shape[1], gallery.k))
+    S = pairs._result(out)
+    if pairs.numel:
+        lib = _lib.load()
+        with torch.cuda.device(pairs.device):
+            _keep(torch.cuda.current_stream(), pairs._tab, pairs.rows._tab, gallery.groups._tab, gallery.codes,
+                  gallery.scales, gallery.q)
+            _lib.check(lib.hypmi_q4_score(
+                _ptr(gallery.codes), _ptr(gallery.scales), _ptr(gallery.q), gallery.k, _ptr(G), ld, pairs.rows._row(0),
+                gallery.groups._row(0), gallery.groups._row(2), pairs._row(0), pairs._row(3), pairs._q4_tests,
+                pairs.rows.num_groups, pairs._n_tasks[2], _ptr(S), engine.stream_ptr()))
+    return S

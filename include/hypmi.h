@@ -33,6 +33,12 @@ extern "C" {
 
 #define HYPMI_MAX_SEG 4
 
+/* Element types of vectors handed to the grouped operators. */
+#define HYPMI_F32 0
+#define HYPMI_F16 1
+#define HYPMI_BF16 2
+#define HYPMI_F64 3
+
 /* Which side of a trial a packed vector is for: enrol-side rows carry [g, q, 1], test-side rows
  * carry [g, 1, q + c], so that a plain dot product of the two is the log-likelihood ratio. */
 #define HYPMI_SIDE_ENROL 0
@@ -517,6 +523,86 @@ int hypmi_score_extract(const float* S, int64_t lds, int64_t ne, int64_t nt, con
                         const int32_t* key_t, const unsigned char* tar, const unsigned char* non,
                         int64_t ldm, float lo, float hi, int nbins, const unsigned char* want, float* out,
                         int64_t cap, unsigned long long* count, void* stream);
+
+/* ---- grouped operators: rows that fall into groups of unequal sizes ----------------------------- */
+
+/* The rows of group e are offsets[e] .. offsets[e + 1] - 1 (int64, device, n_groups + 1 entries, ascending
+ * from 0; groups may be empty), or, where a call takes `order`, the rows order[offsets[e]] ..
+ * order[offsets[e + 1] - 1].  Work is cut into tiles that never cross a group; a call that is cut takes the
+ * prefix sums of its tile counts (int64, device, n_groups + 1 entries from 0) and their total, which is the
+ * size of the launch, so that neither the host nor the device has to wait for the other.  The tables are not
+ * checked on the device: they have to be the ones described.
+ *
+ * Replaces the loops over recordings, conditions or models that call TransformList.predict
+ * (hyperion/transforms/transform_list.py:41-44), PLDA.llr_1vs1 (hyperion/diarization/diar_ahc_plda.py:143)
+ * and np.dot(x.T, x) (hyperion/pdfs/core/normal.py:102-113) once per group. */
+
+/* Weights of hypmi_grouped_affine, laid out once: W [n_groups x d_in x d_out] and b [n_groups x d_out] (NULL:
+ * 0), fp32 on the device, contiguous, into `weights` (hypmi_grouped_weights_bytes) and `columns`
+ * (hypmi_grouped_columns_bytes), both 16-byte aligned. */
+int64_t hypmi_grouped_weights_bytes(int n_groups, int d_in, int d_out);
+int64_t hypmi_grouped_columns_bytes(int n_groups, int d_out);
+int hypmi_grouped_weights(const float* W, const float* b, int n_groups, int d_in, int d_out, void* weights,
+                          void* columns, void* stream);
+
+/* y_r = x_r W_e + b_e for every row r of every group e, and with lnorm != 0 then
+ * y_r <- sqrt(dims[e]) y_r / (|y_r| + 1e-10)  (dims NULL: d_out).  x: rows of d_in elements of x_type
+ * (HYPMI_F32, HYPMI_F16 or HYPMI_BF16), ldx >= d_in, any alignment of the element type.  y: fp32, 16-byte
+ * aligned, ldy a multiple of 4 and at least d_out; columns d_out .. (d_out rounded up to 4) - 1 are set to
+ * zero, rows of no group are left as they are.  With `order` row order[i] of x goes to row order[i] of y; no
+ * row may occur twice.  tiles: prefix sums of ceil(size / tile_rows), tile_rows 16, 64 or 128.  Accurate to
+ * fp32 (fp16-pair products, fp32 accumulation); a row with a NaN or an infinity comes out
+ * without finite values (fp32 rows: as NaN). */
+int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int d_in, const int64_t* offsets,
+                         const int64_t* tiles, int tile_rows, int n_groups, int64_t n_rows, int64_t n_tiles,
+                         const int32_t* order, const void* weights, const void* columns, const int32_t* dims,
+                         int d_out, int lnorm, float* y, int64_t ldy, void* stream);
+
+/* S_e = G1_e G2_e^T for every group e from packed rows (hypmi_prologue; widths up to 512, multiples of 8; rows
+ * 16-byte aligned): n1_e x n2_e scores, row-major without padding, at element block_offsets[e] of S.  tasks:
+ * prefix sums of ceil(n1_e / hypmi_grouped_score_rows(kp)) * ceil(n2_e / hypmi_grouped_score_span()).
+ * hypmi_grouped_score_rows returns 0 for a width without a kernel.  Accuracy as hypmi_score_pair. */
+int hypmi_grouped_score_rows(int kp);
+int hypmi_grouped_score_span(void);
+int hypmi_grouped_score(const float* G1, int64_t ld1, const float* G2, int64_t ld2, int kp, const int64_t* offsets1,
+                        const int64_t* offsets2, const int64_t* block_offsets, const int64_t* tasks, int n_groups,
+                        int64_t n_tasks, float* S, void* stream);
+
+/* C_e = sum_r w_r x_r x_r^T [d x d] and F_e = sum_r w_r x_r [d] over the rows of every group, in float64 (w NULL:
+ * 1; indexed by row of x).  x: HYPMI_F32 or HYPMI_F64.  C [n_groups x d x d] is exactly symmetric, empty groups
+ * are zero, and the sums are added in a fixed order (same bits from run to run).  chunks: prefix sums of
+ * max(1, ceil(size / hypmi_grouped_gram_span())); slots: the same with 0 in place of 1.  workspace:
+ * hypmi_grouped_gram_workspace_bytes(n_slots, d) bytes, 8-byte aligned. */
+int hypmi_grouped_gram_span(void);
+int64_t hypmi_grouped_gram_workspace_bytes(int64_t n_slots, int d);
+int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, int d, const double* w, const int64_t* offsets,
+                           const int64_t* chunks, const int64_t* slots, int n_groups, int64_t n_chunks,
+                           int64_t n_slots, const int32_t* order, double* C, double* F, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---- 4-bit enrolment gallery -------------------------------------------------------------------- */
+
+/* Enrol-side packed rows [g, q, 1] (K = k coordinates) held in 4 bits: per 32 coordinates the scale s is the
+ * smallest bfloat16 number with 7 s >= the largest magnitude and a coordinate is s times the integer nearest to
+ * x / s (halves to even), q stays in fp32.  A coordinate that is not finite makes its row's scores NaN.
+ * Stored in blocks of 64 rows, every group starting a new one: blocks = prefix sums of ceil(size / 64); k-steps
+ * of 32 coordinates = hypmi_q4_ksteps(k) (0: k is not supported, 1 to 512 are).  codes: 1024 bytes per block and
+ * k-step, scales: 128 bytes per block and k-step, q: 256 bytes per block; 16-byte aligned.  (In place of the
+ * float64 rows that hyperion/pdfs/plda/splda.py:306-307 keeps.) */
+int hypmi_q4_ksteps(int k);
+int hypmi_q4_task_rows(void);
+int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* offsets, const int64_t* blocks, int n_groups,
+                  int64_t n_blocks, void* codes, void* scales, float* q, void* stream);
+
+/* Scores of test-side packed rows [g, 1, q + c] against the gallery, group by group: S_e [tests_e x rows_e],
+ * row-major without padding, at element out_offsets[e] of S; each is the fp32-accurate product with the row that
+ * the codes stand for (hyperion/pdfs/plda/splda.py:312-315).  offsets_t delimits the tests, offsets_g the gallery
+ * rows.  tasks: prefix sums of ceil(rows_e / hypmi_q4_task_rows()) * ceil(tests_e / task_tests), task_tests 16,
+ * 32 or 64. */
+int hypmi_q4_score(const void* codes, const void* scales, const float* q, int k, const float* G, int64_t ldg,
+                   const int64_t* offsets_t, const int64_t* offsets_g, const int64_t* blocks,
+                   const int64_t* out_offsets, const int64_t* tasks, int task_tests, int n_groups, int64_t n_tasks,
+                   float* S, void* stream);
 
 #ifdef __cplusplus
 }
