@@ -42,11 +42,15 @@ inline int64_t xcd_grid(int64_t n) { return (n + 7) / 8 * 8; }
 // 2^e as a float, -126 <= e <= 127
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// x -> x0 + x1 with x0 = fp16(x), x1 = fp16(x - x0), four values: |x - x0 - x1| <= 2^-22 |x| while x1 is a
-// normal fp16 number.  An infinity becomes (inf, NaN): its products are NaN.
-__device__ __forceinline__ void split_pair4(f32x4 x, f16x4& x0, f16x4& x1) {
-    x0 = __builtin_convertvector(x, f16x4);
-    x1 = __builtin_convertvector(x - __builtin_convertvector(x0, f32x4), f16x4);
+// x up -> x0 + x1 with x0 = fp16(x up), x1 = fp16(x up - x0), four values and a power of two `up`:
+// |x up - x0 - x1| <= 2^-22 |x up| while x1 is a normal fp16 number.  An infinity becomes (inf, NaN): its products
+// are NaN.  Three instructions a value (v_mul, half a v_cvt_pk_f16_f32, v_fma_mix_f32, half a v_cvt_pk_f16_f32).
+__device__ __forceinline__ void split_pair4(f32x4 x, float up, f16x4& x0, f16x4& x1) {
+    x0 = __builtin_convertvector(x * up, f16x4);
+    f32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fmaf(x[i], up, -(float)x0[i]);
+    x1 = __builtin_convertvector(r, f16x4);
 }
 
 }  // namespace hypmi_detail

@@ -18,6 +18,8 @@
 // powers of two of headroom cost nothing: x1 keeps 2^-33 of the row's largest magnitude.
 #include "grouped.h"
 
+#include <type_traits>
+
 namespace hypmi_detail {
 
 // four coordinates of a row as floats
@@ -68,26 +70,28 @@ struct AffineArgs {
     int lnorm;
 };
 
-// RT row tiles of 16 per workgroup.  Eight waves: RS of them side by side along the rows, 8 / RS along the
-// output columns, two column tiles of 16 each.  Coordinates are taken in chunks of 512 / RT, so that every
-// thread holds sixteen values of a chunk whatever RT is; the chunk at hand sits in LDS as pairs in operand
-// order (lane l of a 16 x 32 tile: row l & 15, coordinates 8 (l >> 4) .. + 7; the row is XORed with
-// 4 (l >> 4) so that the four coordinate groups of a row fall into different banks when they are written),
-// the next one is on its way in registers.
-template <typename XT, int RT, int RS>
-__global__ __launch_bounds__(512) void grouped_affine_kernel(AffineArgs g) {
+// RT row tiles of 16 per workgroup of eight waves, which take two column tiles of 16 each.  Coordinates are taken in
+// chunks of 256 / RT, so that every thread holds eight values of a chunk whatever RT is; the chunk at hand sits in
+// LDS as pairs in operand order (lane l of a 16 x 32 tile: row l & 15, coordinates 8 (l >> 4) .. + 7; the row is
+// XORed with 4 (l >> 4) so that the four coordinate groups of a row fall into different banks when they are written),
+// the next one is on its way in registers.  Memory operations of a wave complete in order, so the weights of a whole
+// chunk are requested before the vectors of the next one: no product waits for a vector that comes from HBM, and two
+// workgroups share a CU, one converting while the other multiplies.
+template <typename XT, int RT>
+__global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(AffineArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int TM = 16 * RT;
-    constexpr int KC = 512 / RT;
+    constexpr int KC = 256 / RT;
     constexpr int NP = sizeof(XT) == 4 ? 2 : 1;  // parts of x
-    constexpr int LPR = RT == 1 ? 32 : 16;       // lanes that load one row
-    constexpr int RPT = RT == 1 ? 1 : RT / 2;    // rows per thread
-    constexpr int F4 = 4 / RPT;                  // groups of four coordinates per thread and row
-    constexpr int CW = 8 / RS, RW = RT / RS, NT = 2;
+    constexpr int LPR = RT == 1 ? 32 : 64 / RT;  // lanes that load one row
+    constexpr int RPT = RT == 1 ? 1 : 2;         // rows per thread
+    constexpr int F4 = 2 / RPT;                  // groups of four coordinates per thread and row
+    constexpr int CW = 8, NT = 2;
     constexpr int KSC = KC / 32;                 // k-steps per chunk
     __shared__ uint4 tile[2][KSC * RT * NP * 64];
-    __shared__ int exps[2][TM];
-    __shared__ int64_t rows[TM];
+    __shared__ int exps[3][TM];  // a chunk's scales are still read while those of the next but one are written
+    __shared__ int lowered[2];  // the chunk for which a scale was lowered last, by buffer
+    __shared__ int rows[TM];
     __shared__ float norm[CW][TM];
 
     const int64_t t = xcd_slot(blockIdx.x, g.n_tiles);
@@ -100,36 +104,34 @@ __global__ __launch_bounds__(512) void grouped_affine_kernel(AffineArgs g) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < TM) {
         const int64_t r = r0 + (tid < nrows ? tid : 0);
-        rows[tid] = g.order ? (int64_t)g.order[r] : r;
+        rows[tid] = g.order ? g.order[r] : (int)r;
     }
     __syncthreads();
 
     // ---- loading side: this thread's rows and coordinates
     const int c = tid % LPR, rg = tid / LPR;
-    const XT* src[RPT];
     int run[RPT];
     f32x4 v[RPT][F4];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-        src[i] = static_cast<const XT*>(g.x) + rows[rg + (512 / LPR) * i] * g.ldx;
-        run[i] = 126;
-    }
+    for (int i = 0; i < RPT; ++i) run[i] = 126;
     auto fetch = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < RPT; ++i)
+        for (int i = 0; i < RPT; ++i) {
+            const XT* src = static_cast<const XT*>(g.x) + (int64_t)rows[rg + (512 / LPR) * i] * g.ldx;
 #pragma unroll
             for (int f = 0; f < F4; ++f) {
                 const int k = k0 + 4 * (c + LPR * f);
                 f32x4 a = {0.f, 0.f, 0.f, 0.f};
                 if (k + 4 <= g.d_in) {
-                    a = Load4<XT>::get(src[i] + k);
+                    a = Load4<XT>::get(src + k);
                 } else if (k < g.d_in) {
-                    for (int q = 0; q < g.d_in - k; ++q) a[q] = (float)src[i][k + q];
+                    for (int q = 0; q < g.d_in - k; ++q) a[q] = (float)src[k + q];
                 }
                 v[i][f] = a;
             }
+        }
     };
-    auto store = [&](int buf) {
+    auto store = [&](int buf, int ch) {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             float m = 0.f;
@@ -140,17 +142,20 @@ __global__ __launch_bounds__(512) void grouped_affine_kernel(AffineArgs g) {
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
             const int ex = __builtin_amdgcn_frexp_expf(m);
-            if (m > 0.f && ex + run[i] > 15) run[i] = 9 - ex;
+            if (m > 0.f && ex + run[i] > 15) {
+                run[i] = 9 - ex;
+                lowered[buf] = ch;
+            }
             const float up = exp2_int(run[i]);
             const int row = rg + (512 / LPR) * i;
-            if (c == 0) exps[buf][row] = run[i];
+            if (c == 0) exps[ch % 3][row] = run[i];
             const int rt = row >> 4, r16 = row & 15;
 #pragma unroll
             for (int f = 0; f < F4; ++f) {
                 const int k = 4 * (c + LPR * f);  // inside the chunk
                 const int s = k >> 5, kq = (k >> 3) & 3, half = (k >> 2) & 1;
                 f16x4 x0, x1;
-                split_pair4(v[i][f] * up, x0, x1);
+                split_pair4(v[i][f], up, x0, x1);
                 f16x4* dst = reinterpret_cast<f16x4*>(
                                  &tile[buf][((s * RT + rt) * NP) * 64 + kq * 16 + (r16 ^ (4 * kq))]) + half;
                 dst[0] = x0;
@@ -159,135 +164,159 @@ __global__ __launch_bounds__(512) void grouped_affine_kernel(AffineArgs g) {
         }
     };
 
-    // ---- computing side
+    // ---- computing side.  Column tiles go round the waves; odd workgroups start at the other end, so that the
+    // waves with a tile more do not all sit on the same SIMD of a CU.
     const int r16 = lane & 15, kq = lane >> 4;
-    const int wr = wave / CW, wc = wave % CW;
+    const int wc = (t & 1) ? CW - 1 - wave : wave;
     const int xs = kq * 16 + (r16 ^ (4 * kq));
-    int ctile[NT];
-    bool live[NT];
-    const uint4* wp[NT];
+    const int ct0 = (int)blockIdx.y * (CW * NT) + wc, ct1 = ct0 + CW;
+    const uint4* wp = g.w + lane;
+    const int64_t w_tile = (int64_t)g.ks * 128;
+    f32x4 acc[RT][NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        ctile[j] = (int)blockIdx.y * (CW * NT) + wc + CW * j;
-        live[j] = ctile[j] < g.ct;
-        wp[j] = g.w + (((int64_t)e * g.ct + (live[j] ? ctile[j] : 0)) * g.ks) * 128 + lane;
-    }
-    f32x4 acc[RW][NT];
-    int cur[RW];
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        cur[i] = 126;
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-
     const int chunks = (g.d_in + KC - 1) / KC;
-    fetch(0);
-    store(0);
-    __syncthreads();
-    for (int ch = 0; ch < chunks; ++ch) {
-        const int buf = ch & 1;
-        if (ch + 1 < chunks) fetch((ch + 1) * KC);
-        if (live[0]) {
-            bool moved = false;
-            int now[RW];
-#pragma unroll
-            for (int i = 0; i < RW; ++i) {
-                now[i] = exps[buf][16 * (wr * RW + i) + r16];
-                moved |= now[i] != cur[i];
-            }
-            if (__any(moved)) {
-#pragma unroll
-                for (int i = 0; i < RW; ++i) {
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[i][j][q] = ldexpf(acc[i][j][q], now[i] - cur[i]);
-                    cur[i] = now[i];
-                }
-            }
-            const int smax = g.ks - ch * KSC < KSC ? g.ks - ch * KSC : KSC;
-            for (int s = 0; s < smax; ++s) {
-                f16x8 w0[NT], w1[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const uint4* p = wp[j] + (int64_t)(ch * KSC + s) * 128;
-                    w0[j] = __builtin_bit_cast(f16x8, p[0]);
-                    w1[j] = __builtin_bit_cast(f16x8, p[64]);
-                }
-#pragma unroll
-                for (int i = 0; i < RW; ++i) {
-                    const uint4* xp = &tile[buf][((s * RT + wr * RW + i) * NP) * 64 + xs];
-                    const f16x8 x0 = __builtin_bit_cast(f16x8, xp[0]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w1[j], x0, acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0[j], x0, acc[i][j], 0, 0, 0);
-                    }
-                    if constexpr (NP == 2) {
-                        const f16x8 x1 = __builtin_bit_cast(f16x8, xp[64]);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0[j], x1, acc[i][j], 0, 0, 0);
-                    }
-                }
-            }
-        }
-        if (ch + 1 < chunks) store(buf ^ 1);
-        __syncthreads();
-    }
 
-    // ---- epilogue: lane holds columns 16 ctile + 4 kq .. + 3 of row 16 (wr RW + i) + r16
+    // the chunk loop of a wave with `tiles` column tiles
+    auto walk = [&](auto tiles_tag) {
+        constexpr int N = decltype(tiles_tag)::value;
+        constexpr int WS = KSC < 4 ? KSC : 4;  // k-steps of weights in registers
+        const uint4* w0p = wp + ((int64_t)e * g.ct + ct0) * w_tile;
+        const uint4* w1p = wp + ((int64_t)e * g.ct + ct1) * w_tile;
+        f16x8 w[WS][N > 0 ? N : 1][2];
+        auto weights = [&](int slot, int s) {
+            s = s < g.ks ? s : g.ks - 1;  // past the end: loaded, not used
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint4* p = (j ? w1p : w0p) + s * 128;
+                w[slot][j][0] = __builtin_bit_cast(f16x8, p[0]);
+                w[slot][j][1] = __builtin_bit_cast(f16x8, p[64]);
+            }
+        };
+        auto step = [&](int buf, int slot, int s) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const uint4* xp = &tile[buf][((s * RT + i) * NP) * 64 + xs];
+                const f16x8 x0 = __builtin_bit_cast(f16x8, xp[0]);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][1], x0, acc[i][j], 0, 0, 0);
+                if constexpr (NP == 2) {
+                    const f16x8 x1 = __builtin_bit_cast(f16x8, xp[64]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x1, acc[i][j], 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x0, acc[i][j], 0, 0, 0);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < WS; ++s) weights(s, s);
+        fetch(0);
+        store(0, 0);
+        __syncthreads();
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int buf = ch & 1;
+            if (ch + 1 < chunks) fetch((ch + 1) * KC);
+            __builtin_amdgcn_sched_barrier(0);
+            if (N > 0) {
+                if (ch > 0 && lowered[buf] == ch) {
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        const int by = exps[ch % 3][16 * i + r16] - exps[(ch + 2) % 3][16 * i + r16];
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) acc[i][j][q] = ldexpf(acc[i][j][q], by);
+                    }
+                }
+                if constexpr (KSC <= 4) {
+#pragma unroll
+                    for (int s = 0; s < KSC; ++s)
+                        if (ch * KSC + s < g.ks) step(buf, s, s);
+                } else {
+                    // a long chunk of few rows: the weights go round a ring of four k-steps
+                    for (int s0 = 0; s0 < KSC; s0 += WS) {
+                        if (ch * KSC + s0 >= g.ks) break;
+#pragma unroll
+                        for (int s = 0; s < WS; ++s) {
+                            if (ch * KSC + s0 + s < g.ks) step(buf, s, s0 + s);
+                            weights(s, ch * KSC + s0 + s + WS);
+                        }
+                    }
+                }
+            }
+            if (ch + 1 < chunks) {
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (KSC <= 4) {
+#pragma unroll
+                    for (int s = 0; s < KSC; ++s) weights(s, (ch + 1) * KSC + s);
+                }
+                store(buf ^ 1, ch + 1);
+            }
+            __syncthreads();
+        }
+    };
+    if (ct1 < g.ct) walk(std::integral_constant<int, 2>());
+    else if (ct0 < g.ct) walk(std::integral_constant<int, 1>());
+    else walk(std::integral_constant<int, 0>());
+
+    // ---- epilogue: lane holds columns 16 ctile + 4 kq .. + 3 of row 16 i + r16
     const int cp = 16 * g.ct;
     const float* col = g.col + (int64_t)e * 2 * cp;
-    float ss[RW];
+    float ss[RT];
 #pragma unroll
-    for (int i = 0; i < RW; ++i) ss[i] = 0.f;
+    for (int i = 0; i < RT; ++i) ss[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        if (!live[j]) continue;
-        const int4 sc = *reinterpret_cast<const int4*>(col + 16 * ctile[j] + 4 * kq);
-        const f32x4 b = *reinterpret_cast<const f32x4*>(col + cp + 16 * ctile[j] + 4 * kq);
+        const int ctile = j ? ct1 : ct0;
+        if (ctile >= g.ct) continue;
+        const int4 sc = *reinterpret_cast<const int4*>(col + 16 * ctile + 4 * kq);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(col + cp + 16 * ctile + 4 * kq);
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
+        for (int i = 0; i < RT; ++i) {
+            const int cur = exps[(chunks - 1) % 3][16 * i + r16];
             // one shift by the sum of both exponents: neither scale alone may leave the range
-            acc[i][j][0] = ldexpf(acc[i][j][0], sc.x - cur[i]) + b[0];
-            acc[i][j][1] = ldexpf(acc[i][j][1], sc.y - cur[i]) + b[1];
-            acc[i][j][2] = ldexpf(acc[i][j][2], sc.z - cur[i]) + b[2];
-            acc[i][j][3] = ldexpf(acc[i][j][3], sc.w - cur[i]) + b[3];
+            acc[i][j][0] = ldexpf(acc[i][j][0], sc.x - cur) + b[0];
+            acc[i][j][1] = ldexpf(acc[i][j][1], sc.y - cur) + b[1];
+            acc[i][j][2] = ldexpf(acc[i][j][2], sc.z - cur) + b[2];
+            acc[i][j][3] = ldexpf(acc[i][j][3], sc.w - cur) + b[3];
 #pragma unroll
             for (int q = 0; q < 4; ++q) ss[i] = fmaf(acc[i][j][q], acc[i][j][q], ss[i]);
         }
     }
-    float factor[RW];
-#pragma unroll
-    for (int i = 0; i < RW; ++i) factor[i] = 1.f;
     if (g.lnorm) {
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
+        for (int i = 0; i < RT; ++i) {
             ss[i] += __shfl_xor(ss[i], 16);
             ss[i] += __shfl_xor(ss[i], 32);
-            if (kq == 0) norm[wc][16 * (wr * RW + i) + r16] = ss[i];
+            if (kq == 0) norm[wc][16 * i + r16] = ss[i];
         }
         __syncthreads();
         const float top = sqrtf((float)(g.dims ? g.dims[e] : g.d_out));
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
+        for (int i = 0; i < RT; ++i) {
             float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < CW; ++w) s += norm[w][16 * (wr * RW + i) + r16];
-            factor[i] = top / (sqrtf(s) + 1e-10f);
+            for (int w = 0; w < CW; ++w) s += norm[w][16 * i + r16];
+            const float factor = top / (sqrtf(s) + 1e-10f);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = acc[i][j] * factor;
         }
     }
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const int row = 16 * (wr * RW + i) + r16;
+    for (int i = 0; i < RT; ++i) {
+        const int row = 16 * i + r16;
         if (row >= nrows) continue;
-        float* out = g.y + rows[row] * g.ldy;
+        float* out = g.y + (int64_t)rows[row] * g.ldy;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int c0 = 16 * ctile[j] + 4 * kq;
-            if (live[j] && c0 < g.cols_y) *reinterpret_cast<f32x4*>(out + c0) = acc[i][j] * factor[i];
+            const int ctile = j ? ct1 : ct0, c0 = 16 * ctile + 4 * kq;
+            if (ctile < g.ct && c0 < g.cols_y) *reinterpret_cast<f32x4*>(out + c0) = acc[i][j];
         }
     }
 #endif
@@ -357,12 +386,12 @@ __global__ __launch_bounds__(256) void grouped_lnorm_kernel(float* __restrict__ 
     for (int k = lane; k < d_out; k += 64) row[k] *= f;
 }
 
-template <typename XT, int RT, int RS>
+template <typename XT, int RT>
 int launch_affine(const AffineArgs& g, hipStream_t stream) {
-    const int per = 2 * (8 / RS);
+    const int per = 16;  // column tiles of a workgroup
     const int64_t gx = xcd_grid(g.n_tiles), gy = (g.ct + per - 1) / per;
     HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
-    hipLaunchKernelGGL((grouped_affine_kernel<XT, RT, RS>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, stream, g);
+    hipLaunchKernelGGL((grouped_affine_kernel<XT, RT>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, stream, g);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
 }
@@ -370,9 +399,9 @@ int launch_affine(const AffineArgs& g, hipStream_t stream) {
 template <typename XT>
 int launch_affine_type(const AffineArgs& g, int tile_rows, hipStream_t stream) {
     switch (tile_rows) {
-        case 16: return launch_affine<XT, 1, 1>(g, stream);
-        case 64: return launch_affine<XT, 4, 1>(g, stream);
-        default: return launch_affine<XT, 8, 1>(g, stream);
+        case 16: return launch_affine<XT, 1>(g, stream);
+        case 64: return launch_affine<XT, 4>(g, stream);
+        default: return launch_affine<XT, 8>(g, stream);
     }
 }
 
@@ -412,6 +441,7 @@ extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int 
                                     const int32_t* dims, int d_out, int lnorm, float* y, int64_t ldy, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     HYPMI_REQUIRE(n_groups >= 0 && n_rows >= 0 && n_tiles >= 0 && d_in > 0 && d_out > 0, "grouped_affine: bad shape");
+    HYPMI_REQUIRE(n_rows <= 0x7fffffffLL, "grouped_affine: at most 2^31 - 1 rows");
     HYPMI_REQUIRE(x_type >= HYPMI_F32 && x_type <= HYPMI_BF16, "grouped_affine: vectors must be fp32, fp16 or bf16");
     HYPMI_REQUIRE(tile_rows == 16 || tile_rows == 64 || tile_rows == 128, "grouped_affine: tiles of 16, 64 or 128 rows");
     const int cols_y = (d_out + 3) / 4 * 4;

@@ -3,17 +3,18 @@
 // hyperion/diarization/diar_ahc_plda.py:131-141, whose statistics are np.dot(x.T, x),
 // hyperion/pdfs/core/normal.py:102-113) or of every domain of a training set, in one pass.
 //
-// What bounds it is the float64 multiply-add: on this chip the vector unit sustains 61 TFLOP/s of v_fma_f64
-// and the float64 matrix instruction 35 (both measured over registers only, together no more than either), so
-// the kernel is written for the vector unit.  A wave owns a 32 x 32 block of C.  Its four 16-lane rows take
-// four consecutive samples; a lane holds two features of the block's row side (a) and two of its column side
-// (b), and v_fmac_f64 with a row broadcast multiplies the a of lane i by every lane's b: four 8-byte loads per
-// lane feed 64 multiply-adds, without shared memory.  The four partial sums (samples modulo four) are added at
-// the end.  Only blocks on or above the diagonal are computed, and both halves are written from them.
+// What bounds it is the float64 matrix instruction: v_mfma_f64_16x16x4 sustains 70 TFLOP/s over registers on this
+// chip (v_fma_f64 55 to 60, with or without row broadcasts; both together no more than either).  A wave owns a
+// 32 x 32 block of C; an operand is four samples of sixteen features, read as it lies in memory: four 8-byte loads
+// per lane feed four instructions of 64 clocks, without shared memory.  Sixteen samples are in flight while the
+// sixteen before them are multiplied.  Only blocks on or above the diagonal are computed (and three quarters of
+// those on it), and both halves are written from them.
 //
 // A group with more than `span` rows is cut into chunks; every chunk writes its block to a slot of the
 // workspace and a second kernel adds the slots in chunk order, so results do not depend on scheduling.
 #include "grouped.h"
+
+#include <type_traits>
 
 namespace hypmi_detail {
 
@@ -37,31 +38,7 @@ struct GramArgs {
 
 constexpr int GRAM_SPAN = 1024;  // rows of one chunk
 
-// acc[i] += a(lane i of this lane's row of 16) * b, i = 0 .. 15.  The leading s_nop covers the two wait states
-// between a vector write of `a` and its use through DPP.
-__device__ __forceinline__ void fma_row16(double (&acc)[16], double a, double b) {
-    asm("s_nop 1\n\t"
-        "v_fmac_f64_dpp %0, %16, %17 row_newbcast:0 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %1, %16, %17 row_newbcast:1 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %2, %16, %17 row_newbcast:2 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %3, %16, %17 row_newbcast:3 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %4, %16, %17 row_newbcast:4 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %5, %16, %17 row_newbcast:5 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %6, %16, %17 row_newbcast:6 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %7, %16, %17 row_newbcast:7 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %8, %16, %17 row_newbcast:8 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %9, %16, %17 row_newbcast:9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %10, %16, %17 row_newbcast:10 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %11, %16, %17 row_newbcast:11 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %12, %16, %17 row_newbcast:12 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %13, %16, %17 row_newbcast:13 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %14, %16, %17 row_newbcast:14 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f64_dpp %15, %16, %17 row_newbcast:15 row_mask:0xf bank_mask:0xf"
-        : "+&v"(acc[0]), "+&v"(acc[1]), "+&v"(acc[2]), "+&v"(acc[3]), "+&v"(acc[4]), "+&v"(acc[5]), "+&v"(acc[6]),
-          "+&v"(acc[7]), "+&v"(acc[8]), "+&v"(acc[9]), "+&v"(acc[10]), "+&v"(acc[11]), "+&v"(acc[12]), "+&v"(acc[13]),
-          "+&v"(acc[14]), "+&v"(acc[15])
-        : "v"(a), "v"(b));
-}
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // block pair p (row-major over bi <= bj) -> bi, bj
 __device__ __forceinline__ void pair_of(int p, int nb, int& bi, int& bj) {
@@ -73,8 +50,15 @@ __device__ __forceinline__ void pair_of(int p, int nb, int& bi, int& bj) {
     bj = bi + p;
 }
 
+// Four steps of four samples; `a` / `b` are the row and the column side of the block.
 template <typename XT>
-__global__ __launch_bounds__(256) void grouped_gram_kernel(GramArgs g) {
+struct GramBatch {
+    XT a[4][2], b[4][2];
+    double w[4];
+};
+
+template <typename XT, bool ORDERED, bool WEIGHTED>
+__global__ __launch_bounds__(256, 2) void grouped_gram_kernel(GramArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int quads = (g.pairs + 3) >> 2;
     const int64_t t = xcd_slot(blockIdx.x, g.n_chunks * quads);
@@ -89,58 +73,98 @@ __global__ __launch_bounds__(256) void grouped_gram_kernel(GramArgs g) {
     const int ns = s_lim - s_beg < GRAM_SPAN ? (int)(s_lim - s_beg) : GRAM_SPAN;
     int bi, bj;
     pair_of(pair, g.nb, bi, bj);
+    const bool diag = bi == bj;
     const int lane = threadIdx.x & 63, l15 = lane & 15, l4 = lane >> 4;
     const XT* X = static_cast<const XT*>(g.x);
-    int fa[2], fb[2];
+    unsigned fa[2], fb[2];  // features of this lane, clamped into the row: those past it are computed and not stored
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        fa[h] = 32 * bi + 16 * h + l15;
-        fb[h] = 32 * bj + 16 * h + l15;
-        fa[h] = fa[h] < g.d ? fa[h] : g.d - 1;
-        fb[h] = fb[h] < g.d ? fb[h] : g.d - 1;
+        const int u = 32 * bi + 16 * h + l15, v = 32 * bj + 16 * h + l15;
+        fa[h] = (unsigned)(u < g.d ? u : g.d - 1);
+        fb[h] = (unsigned)(v < g.d ? v : g.d - 1);
     }
-    double acc[2][2][16];
+    f64x4 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0;
+        for (int j = 0; j < 2; ++j) acc[i][j] = (f64x4){0.0, 0.0, 0.0, 0.0};
     double f[2] = {0.0, 0.0};
 
-    XT a[2], b[2];
-    double ws;
-    auto fetch = [&](int s) {
-        const int64_t r = s_beg + (s + l4 < ns ? s + l4 : ns - 1);
-        const int64_t row = g.order ? (int64_t)g.order[r] : r;
-        const XT* p = X + row * g.ldx;
+    // samples s .. s + 15 of the chunk; in the last batch a sample past the end is a copy of the last one
+    auto fetch = [&](GramBatch<XT>& v, int s, bool last) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            a[h] = p[fa[h]];
-            b[h] = p[fb[h]];
-        }
-        ws = s + l4 < ns ? (g.w ? g.w[row] : 1.0) : 0.0;
-    };
-    if (ns > 0) {
-        fetch(0);
-        for (int s = 0; s < ns; s += 4) {
-            const bool in = s + l4 < ns;  // a row past the end is a copy of the last one: taken out by value
-            double da[2], db[2];
+        for (int k = 0; k < 4; ++k) {
+            int r = s + 4 * k + l4;
+            if (last && r >= ns) r = ns - 1;
+            if constexpr (ORDERED) {
+                const int64_t row = g.order[s_beg + r];
+                const XT* p = X + row * g.ldx;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                da[h] = in ? (double)a[h] : 0.0;
-                db[h] = in ? (g.w ? (double)b[h] * ws : (double)b[h]) : 0.0;
+                for (int h = 0; h < 2; ++h) {
+                    v.a[k][h] = p[fa[h]];
+                    v.b[k][h] = p[fb[h]];
+                }
+                if (WEIGHTED) v.w[k] = g.w[row];
+            } else {
+                const XT* p = X + (s_beg + s + 4 * k) * g.ldx;  // the same for all lanes
+                const int64_t d = (int64_t)(r - s - 4 * k) * g.ldx;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v.a[k][h] = p[d + fa[h]];
+                    v.b[k][h] = p[d + fb[h]];
+                }
+                if (WEIGHTED) v.w[k] = g.w[s_beg + r];
             }
-            if (s + 4 < ns) fetch(s + 4);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) f[h] += db[h];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) fma_row16(acc[i][j], da[i], db[j]);
         }
-    }
-    // the four samples of a step
+    };
+    auto walk = [&](auto diag_tag) {
+        constexpr bool DIAG = decltype(diag_tag)::value;
+        auto multiply = [&](const GramBatch<XT>& v, int s, bool last) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                double da[2], db[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    da[h] = (double)v.a[k][h];
+                    db[h] = (double)v.b[k][h];
+                    if (WEIGHTED) db[h] *= v.w[k];
+                    if (last && s + 4 * k + l4 >= ns) da[h] = db[h] = 0.0;
+                    if (DIAG) f[h] += db[h];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (i <= j || !DIAG)
+                            acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(da[i], db[j], acc[i][j], 0, 0, 0);
+            }
+        };
+        // two batches by turns, so that none is copied: a copy would wait for its loads before the batch at hand
+        // is multiplied
+        GramBatch<XT> u, v;
+        int s = 0;
+        if (ns >= 16) fetch(u, 0, false);
+        for (; s + 32 <= ns; s += 32) {
+            fetch(v, s + 16, false);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(u, s, false);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(u, s + 48 <= ns ? s + 32 : s, false);  // always as many loads: the waits are counted
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(v, s + 16, false);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (s + 16 <= ns) {
+            multiply(u, s, false);
+            s += 16;
+        }
+        if (s < ns) {
+            fetch(v, s, true);
+            multiply(v, s, true);
+        }
+    };
+    if (diag) walk(std::true_type{});
+    else walk(std::false_type{});
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         f[h] += __shfl_xor(f[h], 16);
@@ -154,23 +178,19 @@ __global__ __launch_bounds__(256) void grouped_gram_kernel(GramArgs g) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                double v = acc[i][j][q];
-                v += __shfl_xor(v, 16);
-                v += __shfl_xor(v, 32);
-                // C[32 bi + 16 i + q][32 bj + 16 j + l15]
-                if (l4 != (q & 3)) continue;  // all four rows hold the sum; they share the stores
+            for (int q = 0; q < 4; ++q) {
+                const int rr = 16 * i + l4 + 4 * q, cc = 16 * j + l15;
                 if (slot >= 0) {
-                    part[(16 * i + q) * 32 + 16 * j + l15] = v;
+                    part[rr * 32 + cc] = acc[i][j][q];
                 } else {
-                    const int r = 32 * bi + 16 * i + q, c = 32 * bj + 16 * j + l15;
+                    const int r = 32 * bi + rr, c = 32 * bj + cc;
                     if (r <= c && c < g.d) {
-                        C[(int64_t)r * g.d + c] = v;
-                        if (r < c) C[(int64_t)c * g.d + r] = v;
+                        C[(int64_t)r * g.d + c] = acc[i][j][q];
+                        if (r < c) C[(int64_t)c * g.d + r] = acc[i][j][q];
                     }
                 }
             }
-    if (bi == bj && l4 < 2) {
+    if (diag && l4 < 2) {
         const int c = 32 * bi + 16 * l4 + l15;
         const double v = l4 ? f[1] : f[0];
         if (slot >= 0) g.part_f[slot * 32 * g.nb + c] = v;
@@ -243,10 +263,15 @@ extern "C" int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, in
     const int64_t grid = xcd_grid(n_chunks * ((pairs + 3) / 4));
     const int64_t reduce = n_slots ? (int64_t)n_groups * pairs : 0;
     HYPMI_REQUIRE(grid <= 0x7fffffffLL && reduce <= 0x7fffffffLL, "grouped_gram: too many workgroups");
-    if (x_type == HYPMI_F32)
-        hipLaunchKernelGGL(grouped_gram_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, g);
-    else
-        hipLaunchKernelGGL(grouped_gram_kernel<double>, dim3((unsigned)grid), dim3(256), 0, stream, g);
+    const dim3 blocks((unsigned)grid), threads(256);
+    auto launch = [&](auto type, auto ordered) {
+        typedef decltype(type) XT;
+        constexpr bool O = decltype(ordered)::value;
+        if (w) hipLaunchKernelGGL((grouped_gram_kernel<XT, O, true>), blocks, threads, 0, stream, g);
+        else hipLaunchKernelGGL((grouped_gram_kernel<XT, O, false>), blocks, threads, 0, stream, g);
+    };
+    if (x_type == HYPMI_F32) order ? launch(float(), std::true_type{}) : launch(float(), std::false_type{});
+    else order ? launch(double(), std::true_type{}) : launch(double(), std::false_type{});
     HYPMI_HIP(hipGetLastError());
     if (reduce) {
         hipLaunchKernelGGL(grouped_gram_reduce_kernel, dim3((unsigned)reduce), dim3(256), 0, stream, g);

@@ -93,8 +93,8 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
             if (oct >= 4 * KS) continue;
             const int s = oct >> 2, q = oct & 3;
             f16x4 a0, a1, b0, b1;
-            split_pair4(v[o][0] * f, a0, a1);
-            split_pair4(v[o][1] * f, b0, b1);
+            split_pair4(v[o][0], f, a0, a1);
+            split_pair4(v[o][1], f, b0, b1);
             f16x4* dst = reinterpret_cast<f16x4*>(&tile[buf][((ct * KS + s) * 2) * 64 + q * 16 + (row ^ (8 * (q & 1)))]);
             dst[0] = a0;
             dst[1] = b0;
@@ -138,8 +138,8 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             f16x4 a0, a1, b0, b1;
-            split_pair4(u[s][0] * f, a0, a1);
-            split_pair4(u[s][1] * f, b0, b1);
+            split_pair4(u[s][0], f, a0, a1);
+            split_pair4(u[s][1], f, b0, b1);
             a[i][s][0] = __builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7);
             a[i][s][1] = __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7);
         }
