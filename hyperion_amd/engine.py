@@ -614,5 +614,14 @@ def to_host(t, dtype):
     return out
 
 
-from .grouped import (AffineBank, GroupPairs, Q4Rows, RowGroups, grouped_affine, grouped_gram64,  # noqa: E402,F401
-                      grouped_score, q4_rows, q4_score)
+_GROUPED = ("AffineBank", "GroupPairs", "Q4Rows", "RowGroups", "grouped_affine", "grouped_gram64", "grouped_score",
+            "q4_rows", "q4_score")
+
+
+def __getattr__(name):
+    """The grouped operators (hyperion_amd/grouped.py, which builds on this module) are part of the engine."""
+    if name in _GROUPED:
+        from . import grouped
+
+        return getattr(grouped, name)
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
