@@ -10,10 +10,12 @@
 //
 // A wave keeps 16 RT enrol rows as operands in registers and walks up to `span` test rows of its group in
 // tiles of 32, which the four waves of the workgroup load, convert (a row's largest magnitude over eight
-// lanes) and leave in LDS in operand order; the next tile's values are in flight meanwhile.  Test rows are
+// lanes) and leave in LDS in operand order; the values of the next two tiles are in flight meanwhile.  Test rows are
 // the first operand of the matrix instruction, so a lane ends up with four neighbouring scores of one
 // enrol row.
 #include "grouped.h"
+
+#include <type_traits>
 
 namespace hypmi_detail {
 
@@ -57,22 +59,24 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
 
     // ---- test side: lane loads octets (lane >> 3) + 8 o of row 8 wave + (lane & 7) of a tile
     const int lr = 8 * wave + (lane & 7), lo = lane >> 3;
-    f32x4 v[OCT][2];
-    auto fetch = [&](int c0) {
-        const int j = c0 + lr < ncol ? c0 + lr : ncol - 1;
+    typedef f32x4 Octets[OCT][2];
+    Octets v, u;
+    // Every call issues the same loads, so that the waits for one tile's values are counted past those of the next
+    // and past stores: behind the last row the last row is read again, behind the last octet the last octet (taken
+    // out by value in `store`).
+    int oct_at[OCT];
+#pragma unroll
+    for (int o = 0; o < OCT; ++o) oct_at[o] = 8 * (lo + 8 * o) < g.kp ? 8 * (lo + 8 * o) : g.kp - 8;
+    auto fetch = [&](Octets& v, int tile) {
+        const int j = 32 * tile + lr < ncol ? 32 * tile + lr : ncol - 1;
         const float* p = G2 + j * g.ld2;
 #pragma unroll
         for (int o = 0; o < OCT; ++o) {
-            const int k = 8 * (lo + 8 * o);
-            if (k < g.kp) {
-                v[o][0] = *reinterpret_cast<const f32x4*>(p + k);
-                v[o][1] = *reinterpret_cast<const f32x4*>(p + k + 4);
-            } else {
-                v[o][0] = v[o][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            }
+            v[o][0] = *reinterpret_cast<const f32x4*>(p + oct_at[o]);
+            v[o][1] = *reinterpret_cast<const f32x4*>(p + oct_at[o] + 4);
         }
     };
-    auto store = [&](int buf) {
+    auto store = [&](const Octets& v, int buf) {
         float m = 0.f;
 #pragma unroll
         for (int o = 0; o < OCT; ++o)
@@ -91,10 +95,11 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
         for (int o = 0; o < OCT; ++o) {
             const int oct = lo + 8 * o;
             if (oct >= 4 * KS) continue;
+            const float fo = 8 * oct < g.kp ? f : 0.f;
             const int s = oct >> 2, q = oct & 3;
             f16x4 a0, a1, b0, b1;
-            split_pair4(v[o][0], f, a0, a1);
-            split_pair4(v[o][1], f, b0, b1);
+            split_pair4(v[o][0], fo, a0, a1);
+            split_pair4(v[o][1], fo, b0, b1);
             f16x4* dst = reinterpret_cast<f16x4*>(&tile[buf][((ct * KS + s) * 2) * 64 + q * 16 + (row ^ (8 * (q & 1)))]);
             dst[0] = a0;
             dst[1] = b0;
@@ -103,7 +108,9 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
         }
     };
 
-    fetch(0);
+    fetch(v, 0);
+    fetch(u, 1);
+    __builtin_amdgcn_sched_barrier(0);
 
     // ---- enrol side: a[i][s][part] = coordinates 32 s + 8 kq .. + 7 of row i0 + 16 i + r16
     const int64_t i0 = (i_blk * 4 + wave) * (16 * RT);
@@ -114,20 +121,20 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
         int64_t row = i0 + 16 * i + r16;
         row = row < n1 ? row : n1 - 1;
         const float* p = g.G1 + (g.off1[e] + row) * g.ld1 + 8 * kq;
-        f32x4 u[KS][2];
+        f32x4 x[KS][2];
         float m = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             if (32 * s + 8 * kq < g.kp) {
-                u[s][0] = *reinterpret_cast<const f32x4*>(p + 32 * s);
-                u[s][1] = *reinterpret_cast<const f32x4*>(p + 32 * s + 4);
+                x[s][0] = *reinterpret_cast<const f32x4*>(p + 32 * s);
+                x[s][1] = *reinterpret_cast<const f32x4*>(p + 32 * s + 4);
             } else {
-                u[s][0] = u[s][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                x[s][0] = x[s][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(u[s][h][q]));
+                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(x[s][h][q]));
         }
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
@@ -138,66 +145,88 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             f16x4 a0, a1, b0, b1;
-            split_pair4(u[s][0], f, a0, a1);
-            split_pair4(u[s][1], f, b0, b1);
+            split_pair4(x[s][0], f, a0, a1);
+            split_pair4(x[s][1], f, b0, b1);
             a[i][s][0] = __builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7);
             a[i][s][1] = __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    const bool live = i0 < n1;
-    float* out = g.S + g.blocks[e] + j_beg;
     const int xs = kq * 16 + (r16 ^ (8 * (kq & 1)));
-
-    store(0);
-    __syncthreads();
-    const int tiles = (ncol + 31) / 32;
-    for (int it = 0; it < tiles; ++it) {
+    // result rows of this lane; a row past the end holds the last row's scores (its operand is a copy) and stores
+    // them to the same place, so that no store depends on a comparison
+    float* dst[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t row = i0 + 16 * i + r16;
+        dst[i] = g.S + g.blocks[e] + (row < n1 ? row : n1 - 1) * n2 + j_beg + 4 * kq;
+    }
+    auto multiply = [&](int it, bool whole) {
         const int buf = it & 1;
-        if (it + 1 < tiles) fetch(32 * (it + 1));
-        if (live) {
-            f32x4 acc[RT][2];
+        f32x4 acc[RT][2];
 #pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint4* p = &tile[buf][((c * KS + s) * 2) * 64 + xs];
-                    const f16x8 b0 = __builtin_bit_cast(f16x8, p[0]);
-                    const f16x8 b1 = __builtin_bit_cast(f16x8, p[64]);
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) {
-                        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1, a[i][s][0], acc[i][c], 0, 0, 0);
-                        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][1], acc[i][c], 0, 0, 0);
-                        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][0], acc[i][c], 0, 0, 0);
-                    }
-                }
-            // lane: columns 32 it + 16 c + 4 kq .. + 3 of enrol row i0 + 16 i + r16
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int j = 32 * it + 16 * c + 4 * kq;
-                const int4 cs = *reinterpret_cast<const int4*>(&scale[buf][16 * c + 4 * kq]);
+                const uint4* p = &tile[buf][((c * KS + s) * 2) * 64 + xs];
+                const f16x8 b0 = __builtin_bit_cast(f16x8, p[0]);
+                const f16x8 b1 = __builtin_bit_cast(f16x8, p[64]);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const int64_t row = i0 + 16 * i + r16;
-                    if (row >= n1) continue;
-                    // one shift by the sum of both exponents: neither scale alone may leave the range
-                    const f32x4 r = {ldexpf(acc[i][c][0], -rs[i] - cs.x), ldexpf(acc[i][c][1], -rs[i] - cs.y),
-                                     ldexpf(acc[i][c][2], -rs[i] - cs.z), ldexpf(acc[i][c][3], -rs[i] - cs.w)};
-                    float* dst = out + row * n2 + j;
-                    if (j + 4 <= ncol) {
-                        *reinterpret_cast<f32x4_a4*>(dst) = r;
-                    } else {
+                for (int i = 0; i < RT; ++i)
+                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1, a[i][s][0], acc[i][c], 0, 0, 0);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (j + q < ncol) dst[q] = r[q];
-                    }
+                for (int i = 0; i < RT; ++i)
+                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][1], acc[i][c], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][0], acc[i][c], 0, 0, 0);
+            }
+        // lane: columns 32 it + 16 c + 4 kq .. + 3 of enrol row i0 + 16 i + r16
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int j = 32 * it + 16 * c;
+            const int4 cs = *reinterpret_cast<const int4*>(&scale[buf][16 * c + 4 * kq]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                // one shift by the sum of both exponents: neither scale alone may leave the range
+                const f32x4 r = {ldexpf(acc[i][c][0], -rs[i] - cs.x), ldexpf(acc[i][c][1], -rs[i] - cs.y),
+                                 ldexpf(acc[i][c][2], -rs[i] - cs.z), ldexpf(acc[i][c][3], -rs[i] - cs.w)};
+                if (whole) {
+                    *reinterpret_cast<f32x4_a4*>(dst[i] + j) = r;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (j + 4 * kq + q < ncol) dst[i][j + q] = r[q];
                 }
             }
         }
-        if (it + 1 < tiles) store(buf ^ 1);
+    };
+
+    auto walk = [&](auto live_tag) {
+        constexpr bool LIVE = decltype(live_tag)::value;  // this wave has rows
+        store(v, 0);
+        fetch(v, 2);
+        __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
-    }
+        const int whole = ncol >> 5;
+        for (int it = 0; it < whole; it += 2) {
+            if (LIVE) multiply(it, true);
+            store(u, 1);
+            fetch(u, it + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            if (it + 1 == whole) break;
+            if (LIVE) multiply(it + 1, true);
+            store(v, 0);
+            fetch(v, it + 4);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+        }
+        if (LIVE && 32 * whole < ncol) multiply(whole, false);
+    };
+    if (i0 < n1) walk(std::true_type{});
+    else walk(std::false_type{});
 #endif
 }
 
