@@ -53,4 +53,22 @@ __device__ __forceinline__ void split_pair4(f32x4 x, float up, f16x4& x0, f16x4&
     x1 = __builtin_convertvector(r, f16x4);
 }
 
+// max(x, x of another lane) by a data-parallel-primitive control: 0xB1 lane ^ 1, 0x4E lane ^ 2, 0x141 the mirror
+// image within eight lanes, 0x140 within sixteen, 0x128 lane ^ 8
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float x) {
+    const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true);
+    return fmaxf(x, __int_as_float(y));
+}
+
+// max over the lanes l ^ 16, over l ^ 32 (vector instructions; a shuffle goes through LDS)
+__device__ __forceinline__ float swap16_max(float x) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float swap32_max(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
 }  // namespace hypmi_detail

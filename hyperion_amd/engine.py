@@ -623,5 +623,6 @@ def __getattr__(name):
     if name in _GROUPED:
         from . import grouped
 
-        return getattr(grouped, name)
+        value = globals()[name] = getattr(grouped, name)  # found directly from now on
+        return value
     raise AttributeError("module %r has no attribute %r" % (__name__, name))

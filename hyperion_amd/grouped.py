@@ -8,8 +8,8 @@ can be captured in a HIP graph.  Inputs have to be on one device; the work runs 
 stream."""
 import numpy as np
 
-from . import _lib, engine
-from .engine import _ptr, _torch, round_up
+from . import _lib
+from .engine import _ptr, _torch, require_gpu, round_up
 
 _AFFINE_TILES = (16, 64, 128)
 
@@ -25,7 +25,7 @@ def _ceil(a, b):
 
 
 def _device(device=None):
-    torch = engine.require_gpu()
+    torch = require_gpu()
     d = torch.device("cuda" if device is None else device)
     if d.type != "cuda":
         raise ValueError("the grouped operators work on the GPU, not on %s" % d)
@@ -38,14 +38,36 @@ def _tables(arrays, device):
     return torch.from_numpy(np.ascontiguousarray(np.stack(arrays))).to(device)
 
 
-def _keep(stream, *tensors):
-    """Storage that outlives its last Python reference until `stream` has used it."""
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
+def _run(fn, device, owners, *args):
+    """Calls the library function `fn` with `args` and the current stream of `device`.  owners: the plans whose
+    storage the launch reads; on another stream than the one they were made on their storage is marked as used
+    there, so that dropping a plan does not hand its memory to someone else while the launch is running."""
+    torch = _torch()
+    index = device.index
+    raw = torch._C._cuda_getCurrentRawStream(index)
+    for o in owners:
+        if o._stream != raw:
+            stream = torch.cuda.current_stream(device)
+            for t in o._storage:
+                t.record_stream(stream)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, raw)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, raw)
+    if rc:
+        _lib.check(rc)
 
 
-class RowGroups:
+class _Plan:
+    """Device storage that is made once and read by many launches."""
+
+    def _own(self, *tensors):
+        self._storage = [t for t in tensors if t is not None]
+        self._stream = _torch()._C._cuda_getCurrentRawStream(self.device.index)
+
+
+class RowGroups(_Plan):
     """Rows in groups: group e owns `sizes[e]` consecutive rows (zero is allowed), in order, or, with
     `order`, the rows order[offsets[e]] .. order[offsets[e + 1] - 1]; every row may be listed once.
     sizes: host integers.  order: host or device integers, one per listed row."""
@@ -74,8 +96,16 @@ class RowGroups:
         prefix = [_prefix(_ceil(sizes, t)) for t in _AFFINE_TILES]
         chunks, slots = _prefix(np.maximum(cut, 1)), _prefix(np.where(cut > 1, cut, 0))
         self._tab = _tables([self.offsets] + prefix + [chunks, slots], self.device)
+        base = self._tab.data_ptr()
+        self._rows = [base + 8 * i * (self.num_groups + 1) for i in range(6)]  # device pointers of the tables
         self._n_tiles = dict(zip(_AFFINE_TILES, (int(p[-1]) for p in prefix)))
         self._n_chunks, self._n_slots = int(chunks[-1]), int(slots[-1])
+        self._order_ptr = None if self.order is None else self.order.data_ptr()
+        # rows per workgroup of the affine map: the largest tile that most rows can fill
+        used = int(np.count_nonzero(sizes))
+        mean = self.total / used if used else 0
+        self._affine_tile = 16 if mean <= 16 else 64 if mean <= 1000 else 128
+        self._own(self._tab, self.order)
 
     @classmethod
     def from_ids(cls, ids, num_groups=None, device=None):
@@ -111,12 +141,8 @@ class RowGroups:
                 raise ValueError("order lists a row more than once")
         self.order = order.to(device=self.device, dtype=torch.int32).contiguous()
 
-    def _row(self, i):
-        """Device pointer of table row i: 0 offsets, 1 .. 3 tile prefixes, 4 chunks, 5 slots."""
-        return self._tab.data_ptr() + 8 * i * (self.num_groups + 1)
-
     def _check(self, x, what):
-        if x.device != self.device:
+        if x.get_device() != self.device.index:
             raise ValueError("%s is on %s, its groups are on %s" % (what, x.device, self.device))
         if self.order is None:
             if x.shape[0] != self.total:
@@ -125,7 +151,7 @@ class RowGroups:
             raise ValueError("%s has %d rows, the order names row %d" % (what, x.shape[0], self.num_rows - 1))
 
 
-class GroupPairs:
+class GroupPairs(_Plan):
     """Blocks of scores of two sides that have the same groups: block e is rows.sizes[e] x cols.sizes[e],
     the blocks lie one after the other in a flat result without padding."""
 
@@ -149,10 +175,9 @@ class GroupPairs:
         tabs.append(_prefix(_ceil(n1, self._q4_tests) * _ceil(n2, run)))
         self._n_tasks = [int(t[-1]) for t in tabs]
         self._tab = _tables([self.offsets] + tabs, self.device)
-
-    def _row(self, i):
-        """Device pointer of table row i: 0 block offsets, 1 and 2 score tasks (64 and 128 rows), 3 gallery tasks."""
-        return self._tab.data_ptr() + 8 * i * (self.rows.num_groups + 1)
+        base = self._tab.data_ptr()
+        self._rows = [base + 8 * i * (rows.num_groups + 1) for i in range(4)]  # device pointers of the tables
+        self._own(self._tab)
 
     def block(self, flat, e):
         """Block e of a flat result as a [rows, cols] view."""
@@ -171,7 +196,7 @@ class GroupPairs:
         return out
 
 
-class AffineBank:
+class AffineBank(_Plan):
     """One affine map per group, x -> x W[e] + b[e], laid out for grouped_affine.  W [E, d_in, d_out] and b
     [E, d_out] (or None), host arrays or device tensors of any float type, kept at fp32 accuracy.  dims
     [E] (optional): dimension of every map where they differ; W[e][:, dims[e]:] and b[e][dims[e]:] have to be
@@ -202,10 +227,11 @@ class AffineBank:
         self._w = torch.empty(lib.hypmi_grouped_weights_bytes(*args) // 4, dtype=torch.int32, device=self.device)
         self._c = torch.empty(lib.hypmi_grouped_columns_bytes(self.num_groups, self.d_out) // 4, dtype=torch.float32,
                               device=self.device)
+        self._own(self._w, self._c, self.dims)
+        self._dims_ptr = None if self.dims is None else self.dims.data_ptr()
         if self.num_groups:
-            with torch.cuda.device(self.device):
-                _lib.check(lib.hypmi_grouped_weights(_ptr(W), None if b is None else _ptr(b), *args, _ptr(self._w),
-                                                     _ptr(self._c), engine.stream_ptr()))
+            _run(lib.hypmi_grouped_weights, self.device, (), _ptr(W), None if b is None else _ptr(b), *args,
+                 _ptr(self._w), _ptr(self._c))
 
     def _fp32(self, a):
         torch = _torch()
@@ -216,20 +242,34 @@ class AffineBank:
         return a.to(device=self.device, dtype=torch.float32).contiguous()
 
 
+_KINDS = {}
+
+
+def _kinds(op):
+    """Element types an operator takes -> their numbers in the C ABI."""
+    if not _KINDS:
+        torch = _torch()
+        _KINDS["affine"] = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+        _KINDS["gram"] = {torch.float32: _lib.F32, torch.float64: _lib.F64}
+        _KINDS["rows"] = {torch.float32: _lib.F32}
+    return _KINDS[op]
+
+
 def _device_rows(x, types, what):
     """A 2-D device tensor of one of `types` with unit column stride, as it is; a view with other strides is
     copied.  Returns (x, leading dimension)."""
-    torch = engine.require_gpu()
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    if not isinstance(x, _torch().Tensor) or not x.is_cuda:
         raise ValueError("%s must be a device tensor" % what)
     if x.dim() != 2:
         raise ValueError("%s must be 2-D, got shape %s" % (what, tuple(x.shape)))
     if x.dtype not in types:
         raise ValueError("%s is %s, expected one of %s" % (what, x.dtype, ", ".join(str(t) for t in types)))
     n, d = x.shape
-    if (d > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < d):
+    ld, step = x.stride()
+    if (d > 1 and step != 1) or (n > 1 and ld < d):
         x = x.contiguous()
-    return x, (x.stride(0) if n > 1 else d)
+        ld = d
+    return x, (ld if n > 1 else d)
 
 
 def grouped_affine(x, groups, bank, lnorm=False, out=None):
@@ -237,8 +277,8 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
     y <- sqrt(dim_e) y / (|y| + 1e-10).  x: device fp32, fp16 or bf16 [n, d_in]; returns device fp32
     [n, d_out] (fp32 accuracy).  With an ordered RowGroups row i of the result belongs to row i of x; rows of
     no group are zero in a new result and left alone in `out` (fp32, 16-byte aligned rows)."""
-    torch = engine.require_gpu()
-    kinds = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+    torch = _torch()
+    kinds = _kinds("affine")
     x, ldx = _device_rows(x, kinds, "x")
     groups._check(x, "x")
     if bank.device != groups.device:
@@ -262,25 +302,14 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
             raise ValueError("the last row of out has no room for %d elements" % ld)
         if _overlap(x, y):
             raise ValueError("out must not share memory with x")
-    tile = _affine_tile(groups)
+    tile = groups._affine_tile
     n_tiles = groups._n_tiles[tile]
     if n_tiles:
-        with torch.cuda.device(x.device):
-            stream = torch.cuda.current_stream()
-            _keep(stream, groups._tab, groups.order, bank._w, bank._c, bank.dims)
-            _lib.check(_lib.load().hypmi_grouped_affine(
-                _ptr(x), kinds[x.dtype], ldx, bank.d_in, groups._row(0), groups._row(1 + _AFFINE_TILES.index(tile)),
-                tile, groups.num_groups, groups.total, n_tiles, None if groups.order is None else _ptr(groups.order),
-                _ptr(bank._w), _ptr(bank._c), None if bank.dims is None else _ptr(bank.dims), d, int(bool(lnorm)),
-                _ptr(y), ld if out is None else (y.stride(0) if n > 1 else ld), engine.stream_ptr()))
-    return y[:, :d] if out is None else out
-
-
-def _affine_tile(groups):
-    """Rows per workgroup: the largest tile that most rows can fill."""
-    used = int(np.count_nonzero(groups.sizes))
-    mean = groups.total / used if used else 0
-    return 16 if mean <= 16 else 64 if mean <= 1000 else 128
+        _run(_lib.load().hypmi_grouped_affine, x.device, (groups, bank), x.data_ptr(), kinds[x.dtype], ldx, bank.d_in,
+             groups._rows[0], groups._rows[1 + _AFFINE_TILES.index(tile)], tile, groups.num_groups, groups.total, n_tiles,
+             groups._order_ptr, bank._w.data_ptr(), bank._c.data_ptr(), bank._dims_ptr, d, int(bool(lnorm)),
+             y.data_ptr(), ld if out is None else (y.stride(0) if n > 1 else ld))
+    return (y if ld == d else y[:, :d]) if out is None else out
 
 
 def _overlap(a, b):
@@ -297,8 +326,7 @@ def _overlap(a, b):
 
 def _packed(G, groups, what):
     """Packed rows as the grouped kernels take them: fp32, 16-byte aligned rows."""
-    torch = engine.require_gpu()
-    G, ld = _device_rows(G, (torch.float32,), what)
+    G, ld = _device_rows(G, _kinds("rows"), what)
     groups._check(G, what)
     if G.data_ptr() % 16 or ld % 4:
         raise ValueError("%s must have 16-byte aligned rows" % what)
@@ -320,20 +348,17 @@ def grouped_score(G1, G2, pairs, out=None):
     S = pairs._result(out)
     i = 1 if rows == 64 else 2
     if pairs.numel:
-        torch = _torch()
-        with torch.cuda.device(pairs.device):
-            _keep(torch.cuda.current_stream(), pairs._tab, pairs.rows._tab, pairs.cols._tab)
-            _lib.check(lib.hypmi_grouped_score(_ptr(G1), ld1, _ptr(G2), ld2, kp, pairs.rows._row(0), pairs.cols._row(0),
-                                               pairs._row(0), pairs._row(i), pairs.rows.num_groups,
-                                               pairs._n_tasks[i - 1], _ptr(S), engine.stream_ptr()))
+        _run(lib.hypmi_grouped_score, pairs.device, (pairs, pairs.rows, pairs.cols), G1.data_ptr(), ld1, G2.data_ptr(),
+             ld2, kp, pairs.rows._rows[0], pairs.cols._rows[0], pairs._rows[0], pairs._rows[i], pairs.rows.num_groups,
+             pairs._n_tasks[i - 1], S.data_ptr())
     return S
 
 
 def grouped_gram64(x, groups, w=None):
     """(sum_r w_r x_r x_r^T, sum_r w_r x_r) of every group as device float64 tensors [E, d, d] and [E, d]; x
     device fp32 or float64 [n, d], w optional float64 weights per row of x."""
-    torch = engine.require_gpu()
-    kinds = {torch.float32: _lib.F32, torch.float64: _lib.F64}
+    torch = _torch()
+    kinds = _kinds("gram")
     x, ldx = _device_rows(x, kinds, "x")
     groups._check(x, "x")
     d, E = x.shape[1], groups.num_groups
@@ -350,21 +375,19 @@ def grouped_gram64(x, groups, w=None):
     nbytes = lib.hypmi_grouped_gram_workspace_bytes(groups._n_slots, d)
     ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
     if E:
-        with torch.cuda.device(x.device):
-            _keep(torch.cuda.current_stream(), groups._tab, groups.order)
-            _lib.check(lib.hypmi_grouped_gram_f64(
-                _ptr(x), kinds[x.dtype], ldx, d, None if w is None else _ptr(w), groups._row(0), groups._row(4),
-                groups._row(5), E, groups._n_chunks, groups._n_slots,
-                None if groups.order is None else _ptr(groups.order), _ptr(C), _ptr(F),
-                None if ws is None else _ptr(ws), nbytes, engine.stream_ptr()))
+        _run(lib.hypmi_grouped_gram_f64, x.device, (groups,), x.data_ptr(), kinds[x.dtype], ldx, d,
+             None if w is None else w.data_ptr(), groups._rows[0], groups._rows[4], groups._rows[5], E, groups._n_chunks,
+             groups._n_slots, groups._order_ptr, C.data_ptr(), F.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return C, F
 
 
-class Q4Rows:
+class Q4Rows(_Plan):
     """Packed enrol-side rows held in 4 bits (q4_rows makes them)."""
 
     def __init__(self, codes, scales, q, k, groups):
         self.codes, self.scales, self.q, self.k, self.groups = codes, scales, q, k, groups
+        self.device = codes.device
+        self._own(codes, scales, q)
 
     @property
     def nbytes(self):
@@ -389,8 +412,8 @@ class Q4Rows:
 def q4_rows(G, k, groups=None):
     """Packed enrol-side rows [g, q, 1] (Plan.prologue; k coordinates) -> Q4Rows.  groups: partitions of the
     gallery (default: one)."""
-    torch = engine.require_gpu()
-    G, ld = _device_rows(G, (torch.float32,), "G")
+    torch = require_gpu()
+    G, ld = _device_rows(G, _kinds("rows"), "G")
     if groups is None:
         groups = RowGroups([G.shape[0]], device=G.device)
     groups._check(G, "G")
@@ -405,20 +428,17 @@ def q4_rows(G, k, groups=None):
     scales = torch.empty((nb, ks, 16, 4), dtype=torch.int16, device=G.device)
     q = torch.empty((nb, 64), dtype=torch.float32, device=G.device)
     if nb:
-        with torch.cuda.device(G.device):
-            _keep(torch.cuda.current_stream(), groups._tab)
-            _lib.check(lib.hypmi_q4_rows(_ptr(G), ld, int(k), groups._row(0), groups._row(2), groups.num_groups, nb,
-                                         _ptr(codes), _ptr(scales), _ptr(q), engine.stream_ptr()))
+        _run(lib.hypmi_q4_rows, G.device, (groups,), G.data_ptr(), ld, int(k), groups._rows[0], groups._rows[2],
+             groups.num_groups, nb, codes.data_ptr(), scales.data_ptr(), q.data_ptr())
     return Q4Rows(codes, scales, q, int(k), groups)
 
 
 def q4_score(gallery, G, pairs, out=None):
     """Scores of packed test-side rows [g, 1, q + c] against a 4-bit gallery, group by group: the flat device
     fp32 result of `pairs` = GroupPairs(test groups, gallery.groups); block e is [tests, gallery rows]."""
-    torch = engine.require_gpu()
     if pairs.cols is not gallery.groups and not np.array_equal(pairs.cols.sizes, gallery.groups.sizes):
         raise ValueError("the columns of pairs are not the groups of the gallery")
-    G, ld = _device_rows(G, (torch.float32,), "G")
+    G, ld = _device_rows(G, _kinds("rows"), "G")
     pairs.rows._check(G, "G")
     if gallery.codes.device != pairs.device:
         raise ValueError("the gallery is on %s, the groups on %s" % (gallery.codes.device, pairs.device))
@@ -426,12 +446,9 @@ def q4_score(gallery, G, pairs, out=None):
         raise ValueError("packed rows of %d elements for a gallery of %d coordinates" % (G.shape[1], gallery.k))
     S = pairs._result(out)
     if pairs.numel:
-        lib = _lib.load()
-        with torch.cuda.device(pairs.device):
-            _keep(torch.cuda.current_stream(), pairs._tab, pairs.rows._tab, gallery.groups._tab, gallery.codes,
-                  gallery.scales, gallery.q)
-            _lib.check(lib.hypmi_q4_score(
-                _ptr(gallery.codes), _ptr(gallery.scales), _ptr(gallery.q), gallery.k, _ptr(G), ld, pairs.rows._row(0),
-                gallery.groups._row(0), gallery.groups._row(2), pairs._row(0), pairs._row(3), pairs._q4_tests,
-                pairs.rows.num_groups, pairs._n_tasks[2], _ptr(S), engine.stream_ptr()))
+        groups = gallery.groups
+        _run(_lib.load().hypmi_q4_score, pairs.device, (pairs, pairs.rows, groups, gallery), gallery.codes.data_ptr(),
+             gallery.scales.data_ptr(), gallery.q.data_ptr(), gallery.k, G.data_ptr(), ld, pairs.rows._rows[0],
+             groups._rows[0], groups._rows[2], pairs._rows[0], pairs._rows[3], pairs._q4_tests, pairs.rows.num_groups,
+             pairs._n_tasks[2], S.data_ptr())
     return S
