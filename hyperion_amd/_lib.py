@@ -199,12 +199,11 @@ SIGNATURES = {
                                               c_void_p, ctypes.c_int, i64, i64, c_void_p, c_void_p, c_void_p,
                                               c_void_p, i64, c_void_p]),
     "hypmi_q4_ksteps": (ctypes.c_int, [ctypes.c_int]),
-    "hypmi_q4_task_rows": (ctypes.c_int, []),
     "hypmi_q4_rows": (ctypes.c_int, [c_void_p, i64, ctypes.c_int, c_void_p, c_void_p, ctypes.c_int, i64, c_void_p,
                                      c_void_p, c_void_p, c_void_p]),
     "hypmi_q4_score": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int, c_void_p, i64, c_void_p, c_void_p,
-                                      c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, i64, c_void_p,
-                                      c_void_p]),
+                                      c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, i64,
+                                      c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -28,7 +28,6 @@ namespace hypmi_detail {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int Q4_BLOCK = 64;     // rows of a block
-constexpr int Q4_TASK = 1024;    // gallery rows one workgroup walks
 
 // One thread per (row slot, k-step).
 __global__ __launch_bounds__(256) void q4_rows_kernel(const float* __restrict__ G, int64_t ld, int k, int ks_all,
@@ -96,17 +95,17 @@ struct Q4Args {
     const int64_t* off_g;   // [n_groups + 1] gallery rows
     const int64_t* blk;     // [n_groups + 1] prefix of gallery blocks
     const int64_t* out;     // [n_groups + 1] element offsets of the score blocks
-    const int64_t* tasks;   // [n_groups + 1] prefix of ceil(n / Q4_TASK) * ceil(m / (16 TT))
+    const int64_t* tasks;   // [n_groups + 1] prefix of ceil(n / run_rows) * ceil(m / (16 TT))
     int n_groups;
     int64_t n_tasks;
-    int phases;
+    int phases, run_rows;
     float* S;
 };
 
 // KH k-steps of 32 coordinates are one unit of the walk: what is prefetched and what is unrolled.  A gallery block
 // is `phases` units; up to 192 coordinates it is one.
 template <int KH, int TT>  // TT: tiles of 16 tests
-__global__ __launch_bounds__(256) void q4_score_kernel(Q4Args g) {
+__global__ __launch_bounds__(256, TT == 4 ? 2 : 3) void q4_score_kernel(Q4Args g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     extern __shared__ __attribute__((aligned(16))) uint4 test[];  // [TT][ks][2][64]
     __shared__ __attribute__((aligned(16))) int up_s[16 * TT];
@@ -116,7 +115,7 @@ __global__ __launch_bounds__(256) void q4_score_kernel(Q4Args g) {
     if (t < 0) return;
     const int e = find_group(g.tasks, g.n_groups, t);
     const int64_t n = g.off_g[e + 1] - g.off_g[e], m_all = g.off_t[e + 1] - g.off_t[e];
-    const int64_t runs = (n + Q4_TASK - 1) / Q4_TASK;
+    const int64_t runs = (n + g.run_rows - 1) / g.run_rows;
     const int64_t task = t - g.tasks[e];
     const int64_t tb = task / runs, run = task - tb * runs;
     const int64_t t0 = tb * 16 * TT;
@@ -127,8 +126,8 @@ __global__ __launch_bounds__(256) void q4_score_kernel(Q4Args g) {
     const int ks_all = KH * g.phases;
 
     // ---- gallery blocks of this wave: wave, wave + 4, ... of the run
-    const int64_t row0 = run * Q4_TASK;
-    const int nb = (int)(((n - row0 < Q4_TASK ? n - row0 : Q4_TASK) + Q4_BLOCK - 1) / Q4_BLOCK);
+    const int64_t row0 = run * g.run_rows;
+    const int nb = (int)(((n - row0 < g.run_rows ? n - row0 : g.run_rows) + Q4_BLOCK - 1) / Q4_BLOCK);
     const int64_t b0 = g.blk[e] + row0 / Q4_BLOCK;
     const int units = wave < nb ? ((nb - wave + 3) >> 2) * g.phases : 0;
     uint4 c[KH];
@@ -154,41 +153,58 @@ __global__ __launch_bounds__(256) void q4_score_kernel(Q4Args g) {
     };
     if (units) fetch();
 
-    // ---- tests: wave w prepares tiles w, w + 4, ...; lane holds coordinates 32 ks + 8 kq .. + 7 of test r16
-    for (int tt = wave; tt < TT; tt += 4) {
-        const int ti = 16 * tt + r16;
+    // ---- tests: lane holds coordinates 32 ks + 8 kq .. + 7 of test r16 of a tile.  4 / TT waves share a tile: each
+    // reads all of it (one latency, whatever its width) and prepares every (4 / TT)th k-step.
+    {
+        const int tt = wave % TT, ti = 16 * tt + r16;
         const float* p = g.G + (g.off_t[e] + t0 + (ti < m ? ti : 0)) * g.ld;
         float top = 0.f;
-        for (int ks = 0; ks < ks_all; ++ks)
+        auto coords = [&](int ks, f32x4& lo, f32x4& hi) {
+            const int k = 32 * ks + 8 * kq, at = k < g.k ? k : (g.k - 1) & ~7;
+            lo = *reinterpret_cast<const f32x4*>(p + at);
+            hi = *reinterpret_cast<const f32x4*>(p + at + 4);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = 32 * ks + 8 * kq + j;
-                if (ti < m && k < g.k) top = fmaxf(top, fabsf(p[k]));
+            for (int j = 0; j < 4; ++j) {  // q and the padding of a row lie behind its coordinates
+                lo[j] = (ti < m && k + j < g.k) ? lo[j] : 0.f;
+                hi[j] = (ti < m && k + 4 + j < g.k) ? hi[j] : 0.f;
             }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        };
+#pragma unroll 4
+        for (int ks = 0; ks < ks_all; ++ks) {
+            f32x4 lo, hi;
+            coords(ks, lo, hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(lo[j]), fabsf(hi[j])));
+        }
+        top = swap32_max(swap16_max(top));
         int up = top > 0.f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
         up = up > 126 ? 126 : up;
         const float f = exp2_int(up);
-        for (int ks = 0; ks < ks_all; ++ks) {
-            f16x8 a0, a1;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = 32 * ks + 8 * kq + j;
-                const float x = (ti < m && k < g.k) ? p[k] * f : 0.f;
-                a0[j] = (_Float16)x;
-                a1[j] = (_Float16)(x - (float)a0[j]);
-            }
+        for (int ks = wave / TT; ks < ks_all; ks += 4 / TT) {
+            f32x4 lo, hi;
+            coords(ks, lo, hi);
+            f16x4 l0, l1, h0, h1;
+            split_pair4(lo, f, l0, l1);
+            split_pair4(hi, f, h0, h1);
             uint4* dst = &test[((tt * ks_all + ks) * 2) * 64 + lane];
-            dst[0] = __builtin_bit_cast(uint4, a0);
-            dst[64] = __builtin_bit_cast(uint4, a1);
+            dst[0] = __builtin_bit_cast(uint4, __builtin_shufflevector(l0, h0, 0, 1, 2, 3, 4, 5, 6, 7));
+            dst[64] = __builtin_bit_cast(uint4, __builtin_shufflevector(l1, h1, 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        if (kq == 0) {
+        if (wave < TT && kq == 0) {
             up_s[ti] = -up;
             add_s[ti] = ti < m ? p[g.k + 1] : 0.f;
         }
     }
     __syncthreads();
+
+    const f16x2 lo8 = {(_Float16)-1032.f, (_Float16)-1032.f}, hi8 = {(_Float16)-72.f, (_Float16)-72.f};
+    const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const unsigned exponent = 0x64006400u;  // 1024 twice
+    auto nibbles = [&](unsigned w, unsigned mask) {  // (w & mask) | exponent, in one instruction
+        unsigned r;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(exponent));
+        return __builtin_bit_cast(f16x2, r);
+    };
 
     float* out = g.S + g.out[e] + t0 * n + row0;
     f32x4 acc[TT][4];
@@ -219,14 +235,12 @@ __global__ __launch_bounds__(256) void q4_score_kernel(Q4Args g) {
             float sf[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const f16x2 lo8 = {(_Float16)-1032.f, (_Float16)-1032.f}, hi8 = {(_Float16)-72.f, (_Float16)-72.f};
-                const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
                 const unsigned h = w[u] >> 8;
                 f16x2 o[4];
-                o[0] = __builtin_bit_cast(f16x2, (w[u] & 0x000f000fu) | 0x64006400u) + lo8;
-                o[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w[u] & 0x00f000f0u) | 0x64006400u), sixteenth, hi8);
-                o[2] = __builtin_bit_cast(f16x2, (h & 0x000f000fu) | 0x64006400u) + lo8;
-                o[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (h & 0x00f000f0u) | 0x64006400u), sixteenth, hi8);
+                o[0] = nibbles(w[u], 0x000f000fu) + lo8;
+                o[1] = __builtin_elementwise_fma(nibbles(w[u], 0x00f000f0u), sixteenth, hi8);
+                o[2] = nibbles(h, 0x000f000fu) + lo8;
+                o[3] = __builtin_elementwise_fma(nibbles(h, 0x00f000f0u), sixteenth, hi8);
                 op[u] = __builtin_bit_cast(f16x8, o);
                 const unsigned p = u < 2 ? sc[ks].x : sc[ks].y;
                 sf[u] = __uint_as_float((u & 1) ? p & 0xffff0000u : p << 16);
@@ -304,7 +318,6 @@ static int q4_ksteps(int k) {
 }
 
 extern "C" int hypmi_q4_ksteps(int k) { return q4_ksteps(k); }
-extern "C" int hypmi_q4_task_rows(void) { return Q4_TASK; }
 
 extern "C" int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* offsets, const int64_t* blocks,
                              int n_groups, int64_t n_blocks, void* codes, void* scales, float* q, void* stream_) {
@@ -325,20 +338,22 @@ extern "C" int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* 
 
 extern "C" int hypmi_q4_score(const void* codes, const void* scales, const float* q, int k, const float* G, int64_t ldg,
                               const int64_t* offsets_t, const int64_t* offsets_g, const int64_t* blocks,
-                              const int64_t* out_offsets, const int64_t* tasks, int task_tests, int n_groups,
-                              int64_t n_tasks, float* S, void* stream_) {
+                              const int64_t* out_offsets, const int64_t* tasks, int task_tests, int task_rows,
+                              int n_groups, int64_t n_tasks, float* S, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     const int ks = q4_ksteps(k);
     HYPMI_REQUIRE(ks > 0, "q4_score: %d coordinates (1 to 512)", k);
     HYPMI_REQUIRE(task_tests == 16 || task_tests == 32 || task_tests == 64, "q4_score: 16, 32 or 64 tests per task");
-    HYPMI_REQUIRE(n_groups >= 0 && n_tasks >= 0 && ldg >= k + 2, "q4_score: bad shape");
+    HYPMI_REQUIRE(task_rows > 0 && task_rows % Q4_BLOCK == 0, "q4_score: task_rows must be a multiple of 64");
+    HYPMI_REQUIRE(n_groups >= 0 && n_tasks >= 0, "q4_score: bad shape");
+    HYPMI_REQUIRE(ldg % 4 == 0 && ldg >= k + 2 && ldg >= (k + 7) / 8 * 8, "q4_score: bad leading dimension");
     if (n_tasks == 0) return HYPMI_OK;
     HYPMI_REQUIRE(codes && scales && q && G && offsets_t && offsets_g && blocks && out_offsets && tasks && S,
                   "q4_score: null pointer");
-    HYPMI_REQUIRE(aligned16(codes) && aligned16(scales), "q4_score: buffers must be 16-byte aligned");
+    HYPMI_REQUIRE(aligned16(codes) && aligned16(scales) && aligned16(G), "q4_score: buffers must be 16-byte aligned");
     const int phases = ks <= 6 ? 1 : ks == 16 ? 4 : 2;
     const Q4Args g = {static_cast<const uint4*>(codes), static_cast<const uint2*>(scales), q, G, ldg, k, offsets_t,
-                      offsets_g, blocks, out_offsets, tasks, n_groups, n_tasks, phases, S};
+                      offsets_g, blocks, out_offsets, tasks, n_groups, n_tasks, phases, task_rows, S};
     switch (ks / phases) {
         case 1: return launch_q4_tests<1>(g, task_tests, stream);
         case 2: return launch_q4_tests<2>(g, task_tests, stream);

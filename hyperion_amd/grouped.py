@@ -12,6 +12,7 @@ from . import _lib
 from .engine import _ptr, _torch, require_gpu, round_up
 
 _AFFINE_TILES = (16, 64, 128)
+_Q4_TESTS = (16, 32, 64)
 
 
 def _prefix(counts):
@@ -168,11 +169,17 @@ class GroupPairs(_Plan):
         self.offsets = _prefix(n1 * n2)
         self.numel = int(self.offsets[-1])
         lib = _lib.load()
-        span, run = lib.hypmi_grouped_score_span(), lib.hypmi_q4_task_rows()
-        top = int(n1.max()) if n1.size else 0
-        self._q4_tests = 16 if top <= 16 else 32 if top <= 32 else 64
+        span = lib.hypmi_grouped_score_span()
+        # tests per gallery task: the codes of a row are unpacked once per tile of tests, which costs about as much
+        # as multiplying them with 32 tests
+        cost = [float(np.sum(n2 * _ceil(n1, t) * (32.0 + t))) for t in _Q4_TESTS]
+        self._q4_tests = _Q4_TESTS[int(np.argmin(cost))]
+        # gallery rows per task: three workgroups on each of 256 CUs at once, or a whole number of such rounds
+        work = int(np.sum(n2 * _ceil(n1, self._q4_tests)))
+        rounds = max(1, _ceil(work, 768 * 4096))
+        self._q4_rows = max(256, round_up(_ceil(work, 768 * rounds), 256))
         tabs = [_prefix(_ceil(n1, b) * _ceil(n2, span)) for b in (64, 128)]
-        tabs.append(_prefix(_ceil(n1, self._q4_tests) * _ceil(n2, run)))
+        tabs.append(_prefix(_ceil(n1, self._q4_tests) * _ceil(n2, self._q4_rows)))
         self._n_tasks = [int(t[-1]) for t in tabs]
         self._tab = _tables([self.offsets] + tabs, self.device)
         base = self._tab.data_ptr()
@@ -442,13 +449,19 @@ def q4_score(gallery, G, pairs, out=None):
     pairs.rows._check(G, "G")
     if gallery.codes.device != pairs.device:
         raise ValueError("the gallery is on %s, the groups on %s" % (gallery.codes.device, pairs.device))
-    if G.shape[1] < gallery.k + 2:
-        raise ValueError("packed rows of %d elements for a gallery of %d coordinates" % (G.shape[1], gallery.k))
+    k, width = gallery.k, G.shape[1]
+    if width < k + 2:
+        raise ValueError("packed rows of %d elements for a gallery of %d coordinates" % (width, k))
+    if G.data_ptr() % 16 or ld % 4 or width < round_up(k, 8):  # not as Plan.prologue leaves them: a padded copy
+        ld = round_up(k + 2, 8)
+        buf = _torch().zeros((G.shape[0], ld), dtype=G.dtype, device=G.device)
+        buf[:, :k + 2] = G[:, :k + 2]
+        G = buf
     S = pairs._result(out)
     if pairs.numel:
         groups = gallery.groups
         _run(_lib.load().hypmi_q4_score, pairs.device, (pairs, pairs.rows, groups, gallery), gallery.codes.data_ptr(),
              gallery.scales.data_ptr(), gallery.q.data_ptr(), gallery.k, G.data_ptr(), ld, pairs.rows._rows[0],
-             groups._rows[0], groups._rows[2], pairs._rows[0], pairs._rows[3], pairs._q4_tests, pairs.rows.num_groups,
-             pairs._n_tasks[2], S.data_ptr())
+             groups._rows[0], groups._rows[2], pairs._rows[0], pairs._rows[3], pairs._q4_tests, pairs._q4_rows,
+             pairs.rows.num_groups, pairs._n_tasks[2], S.data_ptr())
     return S

@@ -590,19 +590,19 @@ int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, int d, const 
  * k-step, scales: 128 bytes per block and k-step, q: 256 bytes per block; 16-byte aligned.  (In place of the
  * float64 rows that hyperion/pdfs/plda/splda.py:306-307 keeps.) */
 int hypmi_q4_ksteps(int k);
-int hypmi_q4_task_rows(void);
 int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* offsets, const int64_t* blocks, int n_groups,
                   int64_t n_blocks, void* codes, void* scales, float* q, void* stream);
 
 /* Scores of test-side packed rows [g, 1, q + c] against the gallery, group by group: S_e [tests_e x rows_e],
  * row-major without padding, at element out_offsets[e] of S; each is the fp32-accurate product with the row that
  * the codes stand for (hyperion/pdfs/plda/splda.py:312-315).  offsets_t delimits the tests, offsets_g the gallery
- * rows.  tasks: prefix sums of ceil(rows_e / hypmi_q4_task_rows()) * ceil(tests_e / task_tests), task_tests 16,
- * 32 or 64. */
+ * rows.  G: 16-byte aligned rows, ldg a multiple of 4, at least k + 2 and at least k rounded up to 8 readable.
+ * tasks: prefix sums of ceil(rows_e / task_rows) * ceil(tests_e / task_tests), task_tests 16, 32 or 64, task_rows
+ * any multiple of 64. */
 int hypmi_q4_score(const void* codes, const void* scales, const float* q, int k, const float* G, int64_t ldg,
                    const int64_t* offsets_t, const int64_t* offsets_g, const int64_t* blocks,
-                   const int64_t* out_offsets, const int64_t* tasks, int task_tests, int n_groups, int64_t n_tasks,
-                   float* S, void* stream);
+                   const int64_t* out_offsets, const int64_t* tasks, int task_tests, int task_rows, int n_groups,
+                   int64_t n_tasks, float* S, void* stream);
 
 #ifdef __cplusplus
 }

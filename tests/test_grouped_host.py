@@ -73,10 +73,11 @@ def test_refusals_of_the_c_abi():
     assert "bad shape" in _refused("hypmi_q4_rows", P, 30, 30, P, P, 1, 1, P, P, P, None)
     assert "null" in _refused("hypmi_q4_rows", P, 32, 30, P, P, 1, 1, None, P, P, None)
 
-    def q4(codes=P, k=30, ld=32, tests=16):
-        return _refused("hypmi_q4_score", codes, P, P, k, P, ld, P, P, P, P, P, tests, 1, 1, P, None)
+    def q4(codes=P, k=30, ld=32, tests=16, rows=64):
+        return _refused("hypmi_q4_score", codes, P, P, k, P, ld, P, P, P, P, P, tests, rows, 1, 1, P, None)
 
-    assert "null" in q4(codes=None) and "bad shape" in q4(ld=31)
+    assert "null" in q4(codes=None) and "leading" in q4(ld=31) and "leading" in q4(ld=34) and "leading" in q4(k=33, ld=36)
+    assert "multiple of 64" in q4(rows=96) and "multiple of 64" in q4(rows=0)
     assert "16, 32 or 64" in q4(tests=48) and "coordinates" in q4(k=0)
     assert "16-byte" in q4(codes=ctypes.c_void_p(8))
 
@@ -86,4 +87,4 @@ def test_nothing_to_do_is_no_error():
     assert lib.hypmi_grouped_affine(None, 0, 8, 8, None, None, 64, 0, 0, 0, None, None, None, None, 4, 0, None, 4, None) == 0
     assert lib.hypmi_grouped_score(None, 40, None, 40, 40, None, None, None, None, 0, 0, None, None) == 0
     assert lib.hypmi_grouped_gram_f64(None, 0, 8, 8, None, None, None, None, 0, 0, 0, None, None, None, None, 0, None) == 0
-    assert lib.hypmi_q4_score(None, None, None, 30, None, 32, None, None, None, None, None, 16, 0, 0, None, None) == 0
+    assert lib.hypmi_q4_score(None, None, None, 30, None, 32, None, None, None, None, None, 16, 64, 0, 0, None, None) == 0
