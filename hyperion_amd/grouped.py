@@ -177,7 +177,7 @@ class GroupPairs(_Plan):
         # gallery rows per task: three workgroups on each of 256 CUs at once, or a whole number of such rounds
         work = int(np.sum(n2 * _ceil(n1, self._q4_tests)))
         rounds = max(1, _ceil(work, 768 * 4096))
-        self._q4_rows = max(256, round_up(_ceil(work, 768 * rounds), 256))
+        self._q4_rows = max(256, round_up(_ceil(work, 768 * rounds), 64))
         tabs = [_prefix(_ceil(n1, b) * _ceil(n2, span)) for b in (64, 128)]
         tabs.append(_prefix(_ceil(n1, self._q4_tests) * _ceil(n2, self._q4_rows)))
         self._n_tasks = [int(t[-1]) for t in tabs]
