@@ -386,6 +386,41 @@ __global__ __launch_bounds__(256) void grouped_lnorm_kernel(float* __restrict__ 
     for (int k = lane; k < d_out; k += 64) row[k] *= f;
 }
 
+// Packing of projected rows by the maps of their group: g_k = (s_k + shift_t[k]) scale_t[k],
+// h_k = (s_k + shift_n[k]) scale_n[k], q = (|g|^2 - |h|^2) / 2 into an enrol-side row [g, q, 1] and a test-side row
+// [g, 1, q + c] (book_pack_kernel's arithmetic with maps [n_groups][4][K] and constants c[n_groups]).  One wave per
+// row; either side may be left out.
+__global__ __launch_bounds__(256) void grouped_pack_kernel(const float* __restrict__ s, int64_t lds, int K,
+                                                           const int64_t* __restrict__ offsets, int n_groups,
+                                                           int64_t n, const float* __restrict__ maps,
+                                                           const float* __restrict__ c, float* __restrict__ G1,
+                                                           float* __restrict__ G2, int kp) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= n) return;
+    const int lane = threadIdx.x & 63;
+    const int e = find_group(offsets, n_groups, r);
+    const float* m = maps + (int64_t)e * 4 * K;
+    const float* row = s + r * lds;
+    float* out1 = G1 ? G1 + r * kp : nullptr;
+    float* out2 = G2 ? G2 + r * kp : nullptr;
+    float sum = 0.f;
+    for (int k = lane; k < K; k += 64) {
+        const float v = row[k];
+        const float g = (v + m[k]) * m[K + k], h = (v + m[2 * K + k]) * m[3 * K + k];
+        sum += (g - h) * (g + h);
+        if (out1) out1[k] = g;
+        if (out2) out2[k] = g;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const float q = 0.5f * sum;
+    for (int k = K + lane; k < kp; k += 64) {
+        const int j = k - K;
+        if (out1) out1[k] = j == 0 ? q : j == 1 ? 1.f : 0.f;
+        if (out2) out2[k] = j == 0 ? 1.f : j == 1 ? q + c[e] : 0.f;
+    }
+}
+
 template <typename XT, int RT>
 int launch_affine(const AffineArgs& g, hipStream_t stream) {
     const int per = 16;  // column tiles of a workgroup
@@ -464,6 +499,21 @@ extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int 
     HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_affine: too many rows");
     hipLaunchKernelGGL(grouped_lnorm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, y, ldy, d_out, offsets,
                        n_groups, order, dims, n_rows);
+    HYPMI_HIP(hipGetLastError());
+    return HYPMI_OK;
+}
+
+extern "C" int hypmi_grouped_pack(const float* s, int64_t lds, int K, const int64_t* offsets, int n_groups, int64_t n_rows,
+                                  const float* maps, const float* c, float* G1, float* G2, int kp, void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    HYPMI_REQUIRE(K > 0 && kp >= K + 2 && lds >= K && n_groups >= 0 && n_rows >= 0, "grouped_pack: bad shape");
+    HYPMI_REQUIRE(G1 || G2, "grouped_pack: no result asked for");
+    if (n_rows == 0) return HYPMI_OK;
+    HYPMI_REQUIRE(s && offsets && maps && c, "grouped_pack: null pointer");
+    const int64_t blocks = (n_rows + 3) / 4;
+    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_pack: too many rows");
+    hipLaunchKernelGGL(grouped_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, s, lds, K, offsets, n_groups,
+                       n_rows, maps, c, G1, G2, kp);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
 }

@@ -94,10 +94,83 @@ class DiarAHCPLDA:
             plda_model = plda_model.project(pca.T, pca.mu)
         return plda_model.llr_1vs1(x, x, refine=True)
 
+    @staticmethod
+    @engine.small_host_algebra
+    def _recording_models(C, F, sizes, plda_model, pca_var_r):
+        """The PCA of every recording from its moments (host float64 [E, d, d], [E, d]) and the model projected
+        onto it, as padded parameters of three device steps: (W1, b1, dims) of the projection, (W2, b2) of the
+        model's basis, (maps, c) of the packing."""
+        E, d = F.shape
+        firsts, folds = [], []
+        for e in range(E):
+            mu = F[e] / sizes[e]
+            pca = PCA(pca_var_r=pca_var_r, whiten=True)
+            pca.fit(mu=mu, S=C[e] / sizes[e] - np.outer(mu, mu))
+            model = plda_model.project(pca.T, pca.mu)
+            model._validate_for_scoring()
+            firsts.append((pca.T, -(pca.mu @ pca.T)))
+            folds.append((model._shared_fold(), float(model._fold()[4])))
+        dims = np.array([T.shape[1] for T, _ in firsts])
+        D, K = int(dims.max()), folds[0][0]["P"].shape[1]
+        W1, b1 = np.zeros((E, d, D), np.float32), np.zeros((E, D), np.float32)
+        W2, b2 = np.zeros((E, D, K), np.float32), np.zeros((E, K), np.float32)
+        maps, c = np.zeros((E, 4, K), np.float32), np.zeros(E, np.float32)
+        for e, ((T, b), (f, ce)) in enumerate(zip(firsts, folds)):
+            k = dims[e]
+            W1[e, :, :k], b1[e, :k] = T, b
+            W2[e, :k], b2[e] = f["P"], f["pb"]
+            maps[e] = f["shift_t"], f["scale_t"], f["shift_n"], f["scale_n"]
+            c[e] = ce
+        return W1, b1, dims, W2, b2, maps, c
+
+    def scores_batch(self, xs):
+        """Self-score matrices of a batch of recordings, each [segments, dim]: a list of device tensors
+        [n, n], views of one buffer.  The steps of `scores` (without its float64 refinement: entries that cancel
+        to about zero carry an absolute error of some 1e-6 of the terms they are the difference of), every step
+        one launch over all recordings: moments, projection with length normalisation, model basis, packing and
+        the blocks of scores.  A recording needs two segments where a PCA is fitted on it."""
+        torch = engine.require_gpu()
+        xs = [engine.upload(x) for x in xs]
+        if not xs:
+            return []
+        if len({x.shape[1] for x in xs}) != 1:
+            raise ValueError("the recordings have vectors of different dimensions")
+        sizes = [int(x.shape[0]) for x in xs]
+        x = engine.upload(torch.cat(xs))
+        if self.preproc is not None:
+            x = self.preproc.predict(x)
+        groups = engine.RowGroups(sizes)
+        pairs = engine.GroupPairs(groups, groups)
+        if self.pca_var_r < 1:
+            if min(sizes) < 2:
+                raise ValueError("a PCA needs recordings of at least two segments")
+            C, F = engine.grouped_gram64(x, groups)
+            W1, b1, dims, W2, b2, maps, c = self._recording_models(C.cpu().numpy(), F.cpu().numpy(), sizes,
+                                                                  self.plda_model, self.pca_var_r)
+            z = engine.grouped_affine(x, groups, engine.AffineBank(W1, b1, dims=dims), lnorm=True)
+            s = engine.grouped_affine(z, groups, engine.AffineBank(W2, b2))
+            G1, G2 = engine.grouped_pack(s, groups, maps, c)
+        else:
+            plan = self.plda_model.score_plan()
+            G1, G2 = plan.prologue(x, engine.SIDE_ENROL), plan.prologue(x, engine.SIDE_TEST)
+        return pairs.blocks(engine.grouped_score(G1, G2, pairs))
+
+    def cluster_batch(self, xs):
+        """`cluster` for a batch of recordings, scored together (scores_batch): a list of cluster ids per segment.
+        A recording of fewer than two segments is one cluster."""
+        xs = list(xs)
+        many = [i for i, x in enumerate(xs) if x.shape[0] > 1]
+        ids = [np.zeros(x.shape[0], dtype=int) for x in xs]
+        for i, scores in zip(many, self.scores_batch([xs[i] for i in many])):
+            ids[i] = self._cluster_scores(scores)
+        return ids
+
     def cluster(self, x, hist_file=None):
         """x [segments, dim] -> cluster id per segment (host int array).  hist_file (a plot in the
         reference) is ignored."""
-        scores = self.scores(x)
+        return self._cluster_scores(self.scores(x))
+
+    def _cluster_scores(self, scores):
         if self.do_unsup_cal:
             _, bic, _ = self._unsup_gmm_calibration(scores)
             if self.use_bic and bic < 0:  # one Gaussian is enough: target trials only

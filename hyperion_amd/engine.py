@@ -614,8 +614,8 @@ def to_host(t, dtype):
     return out
 
 
-_GROUPED = ("AffineBank", "GroupPairs", "Q4Rows", "RowGroups", "grouped_affine", "grouped_gram64", "grouped_score",
-            "q4_rows", "q4_score")
+_GROUPED = ("AffineBank", "GroupPairs", "Q4Rows", "RowGroups", "grouped_affine", "grouped_gram64", "grouped_pack",
+            "grouped_score", "q4_rows", "q4_score")
 
 
 def __getattr__(name):

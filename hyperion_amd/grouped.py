@@ -340,6 +340,32 @@ def _packed(G, groups, what):
     return G, ld
 
 
+def grouped_pack(s, groups, maps, c, sides="both"):
+    """Packed rows of the projected rows s [n, K] (device fp32, in group order) by the maps of their group: maps
+    [E, 4, K] = shift_t, scale_t, shift_n, scale_n, c [E] (host or device).  Returns (enrol-side, test-side) rows
+    [n, kp]; sides "enrol" or "test": the other is None."""
+    torch = _torch()
+    s, ld = _device_rows(s, _kinds("rows"), "s")
+    groups._check(s, "s")
+    if groups.order is not None:
+        raise ValueError("packing needs rows in group order (RowGroups without order)")
+    if sides not in ("both", "enrol", "test"):
+        raise ValueError("sides must be both, enrol or test")
+    n, K = s.shape
+    maps, c = (torch.as_tensor(a).to(device=s.device, dtype=torch.float32).contiguous() for a in (maps, c))
+    if tuple(maps.shape) != (groups.num_groups, 4, K) or tuple(c.shape) != (groups.num_groups,):
+        raise ValueError("maps must be [%d, 4, %d] and c [%d]" % (groups.num_groups, K, groups.num_groups))
+    lib = _lib.load()
+    kp = lib.hypmi_packed_width(K)
+    G1, G2 = (torch.empty((n, kp), dtype=torch.float32, device=s.device) if sides in ("both", side) else None
+              for side in ("enrol", "test"))
+    if n:
+        _run(lib.hypmi_grouped_pack, s.device, (groups,), s.data_ptr(), ld, K, groups._rows[0], groups.num_groups, n,
+             maps.data_ptr(), c.data_ptr(), None if G1 is None else G1.data_ptr(),
+             None if G2 is None else G2.data_ptr(), kp)
+    return G1, G2
+
+
 def grouped_score(G1, G2, pairs, out=None):
     """Scores of packed enrol rows against packed test rows of the same group (Plan.prologue, both [n, kp]):
     the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e)."""

@@ -558,6 +558,13 @@ int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int d_in, const
                          const int32_t* order, const void* weights, const void* columns, const int32_t* dims,
                          int d_out, int lnorm, float* y, int64_t ldy, void* stream);
 
+/* Packed rows of projected rows s [n_rows x lds] by the maps of their group (hypmi_book_pack with maps
+ * [n_groups x 4 x K] = shift_t, scale_t, shift_n, scale_n and constants c [n_groups], fp32 on the device; rows in
+ * group order): enrol-side rows into G1, test-side rows into G2, [n_rows x kp] each, either NULL.  The packing of
+ * llr_1vs1 for a model per recording (hyperion/diarization/diar_ahc_plda.py:131-143). */
+int hypmi_grouped_pack(const float* s, int64_t lds, int K, const int64_t* offsets, int n_groups, int64_t n_rows,
+                       const float* maps, const float* c, float* G1, float* G2, int kp, void* stream);
+
 /* S_e = G1_e G2_e^T for every group e from packed rows (hypmi_prologue; widths up to 512, multiples of 8; rows
  * 16-byte aligned): n1_e x n2_e scores, row-major without padding, at element block_offsets[e] of S.  tasks:
  * prefix sums of ceil(n1_e / hypmi_grouped_score_rows(kp)) * ceil(n2_e / hypmi_grouped_score_span()).

@@ -1,0 +1,251 @@
+"""What the grouped operators and the 4-bit gallery are for: a batch of recordings diarized together, chains that
+depend on a vector's domain, identification among enrolled vectors.  Scores are held to the bar of the parity tests,
+1e-4 max(|s|, 1), unless a narrower or wider one follows from the format."""
+import numpy as np
+import pytest
+
+import synth
+from conftest import model_from
+
+pytestmark = pytest.mark.gpu
+
+
+def _recordings(model, sizes, seed):
+    rng = np.random.RandomState(seed)
+    chol = np.linalg.cholesky(np.linalg.inv(model["W"])).T
+    d, K = model["mu"].shape[0], model["V"].shape[0]
+    xs = []
+    for n in sizes:
+        spk = rng.randint(0, 1 + n // 12, n)
+        xs.append(model["mu"] + (1.5 * rng.randn(spk.max(initial=0) + 1, K))[spk] @ model["V"] + rng.randn(n, d) @ chol)
+    return xs
+
+
+@pytest.mark.parametrize("var_r", [1, 0.85])
+def test_batch_of_recordings_matches_one_by_one(var_r):
+    from hyperion_amd.diarization import DiarAHCPLDA
+    from hyperion_amd.pdfs.plda import SPLDA
+    from hyperion_amd.transforms import LNorm
+
+    m = synth.make_splda(64, 20)
+    diar = DiarAHCPLDA(SPLDA(mu=m["mu"], V=m["V"], W=m["W"]), preproc=LNorm(), threshold=0.0, pca_var_r=var_r)
+    xs = _recordings(m, [150, 65, 12, 300, 131], 3)
+    for x, got in zip(xs, diar.scores_batch(xs)):
+        want = diar.scores(x).cpu().numpy()
+        got = got.cpu().numpy()
+        assert got.shape == want.shape
+        assert (np.abs(got - want) <= 1e-4 * np.maximum(np.abs(want), 1)).all()
+    xs = xs + [xs[0][:1], xs[0][:0]]
+    ids = diar.cluster_batch(xs)
+    for x, got in zip(xs[:5], ids):
+        assert np.array_equal(got, diar.cluster(x))
+    assert ids[5].tolist() == [0] and ids[6].tolist() == []
+    assert diar.cluster_batch([]) == [] and diar.cluster_batch(xs[5:])[0].tolist() == [0]
+    if var_r < 1:
+        with pytest.raises(ValueError, match="two segments"):
+            diar.scores_batch(xs)
+    with pytest.raises(ValueError, match="different dimensions"):
+        diar.scores_batch([xs[0], xs[1][:, :60]])
+
+
+@pytest.mark.parametrize("tag,var_r,thr", (("full", 1, 4.0), ("pca", 0.8, 2.0)))
+def test_batch_matches_reference(golden, tag, var_r, thr):
+    from hyperion_amd.diarization import DiarAHCPLDA
+    from hyperion_amd.pdfs.plda import SPLDA
+    from hyperion_amd.transforms import LNorm
+
+    g = golden("diarization")
+    m = model_from(g, "m_", "splda")
+    diar = DiarAHCPLDA(SPLDA(mu=m["mu"], V=m["V"], W=m["W"]), preproc=LNorm(), threshold=thr, pca_var_r=var_r)
+    for ids in diar.cluster_batch([g["x"], g["x"][::-1], g["x"]])[::2]:
+        assert np.array_equal(ids, g["ids_" + tag])
+
+
+def test_batch_with_calibration():
+    """do_unsup_cal / use_bic decide per recording, as they do one by one."""
+    from hyperion_amd.diarization import DiarAHCPLDA
+    from hyperion_amd.pdfs.plda import SPLDA
+
+    m = synth.make_splda(40, 10)
+    diar = DiarAHCPLDA(SPLDA(mu=m["mu"], V=m["V"], W=m["W"]), threshold=0.0, do_unsup_cal=True, use_bic=True)
+    xs = _recordings(m, [11, 80, 60], 5)
+    for x, ids in zip(xs, diar.cluster_batch(xs)):
+        assert np.array_equal(ids, diar.cluster(x))
+
+
+def _chains(d, lda, E, seed):
+    from hyperion_amd.transforms import LDA, CentWhiten, LNorm, TransformList
+
+    rng = np.random.RandomState(seed)
+    chains = []
+    for e in range(E):
+        mid = d - 3 * e  # dimensions in between may differ
+        chains.append(TransformList([CentWhiten(mu=rng.randn(d), T=rng.randn(d, mid) / np.sqrt(d)), LNorm(),
+                                     LDA(mu=rng.randn(mid) * 0.1, T=rng.randn(mid, lda) / np.sqrt(mid)), LNorm()]))
+    return chains
+
+
+def test_transform_bank_matches_the_chains():
+    import torch
+
+    from hyperion_amd import engine
+    from hyperion_amd.transforms import LNorm, TransformBank
+
+    E, d, lda, n = 5, 96, 37, 1500
+    chains = _chains(d, lda, E, 1)
+    bank = TransformBank(chains)
+    rng = np.random.RandomState(2)
+    ids = rng.choice([0, 1, 2, 4], n)  # one domain has no vector
+    x = rng.randn(n, d) * 3
+    y = bank.predict(x, ids)
+    assert isinstance(y, np.ndarray) and y.shape == (n, lda) and y.dtype == chains[0].predict(x[:1]).dtype
+    for e in range(E):
+        if (ids == e).any():
+            want = chains[e].predict(x[ids == e])
+            assert (np.abs(y[ids == e] - want) <= 1e-4 * np.maximum(np.abs(want), 1)).all()
+    dev = torch.from_numpy(x).float().cuda()
+    got = bank.predict(dev, engine.RowGroups.from_ids(ids, E))
+    assert got.is_cuda and torch.equal(got, bank.predict(dev, ids))
+    assert np.abs(got.cpu().numpy() - y).max() <= 1e-5
+    # vectors in 16 bits are taken as they are
+    half = bank.predict(dev.bfloat16(), ids)
+    assert torch.equal(half, bank.predict(dev.bfloat16().float(), ids)) or \
+        (half - bank.predict(dev.bfloat16().float(), ids)).abs().max() <= 1e-5
+    # a chain whose parameters change is laid out again
+    chains[0].transforms[0].mu = chains[0].transforms[0].mu + 1
+    z = bank.predict(x, ids)
+    assert np.array_equal(z[ids != 0], y[ids != 0])
+    assert np.abs(z[ids == 0] - chains[0].predict(x[ids == 0])).max() <= 1e-4 * np.abs(z).max()
+    only = TransformBank([LNorm(), LNorm()]).predict(x, ids % 2)
+    assert np.abs(only - LNorm().predict(x)).max() <= 1e-5 * np.abs(only).max()
+    for bad, match in ((lambda: bank.predict(x, ids[:-1]), "group ids for"), (lambda: bank.predict(x, ids + 1), "lie in"),
+                       (lambda: TransformBank([]), "at least one"), (lambda: bank.predict(x[0], ids), "num_vectors, dim"),
+                       (lambda: TransformBank([chains[0], LNorm()]).predict(x, ids % 2), "different"),
+                       (lambda: TransformBank([chains[0], chains[1].transforms[:2]]).predict(x, ids % 2), "different")):
+        with pytest.raises(ValueError, match=match):
+            bad()
+
+
+def _model():
+    from hyperion_amd.pdfs.plda import SPLDA
+
+    m = synth.make_splda(100, 70)
+    return m, SPLDA(mu=m["mu"], V=m["V"], W=m["W"])
+
+
+def _bound(plan, x, xt):
+    """Half a scale per coordinate times the test's projection: what rounding the enrolled side to 4 bits can move."""
+    import torch
+
+    from hyperion_amd import engine
+
+    G1 = plan.prologue(engine.upload(x), engine.SIDE_ENROL)[:, :plan.k].double()
+    G2 = plan.prologue(engine.upload(xt), engine.SIDE_TEST)[:, :plan.k].double().abs()
+    bound = torch.zeros(len(x), len(xt), dtype=torch.float64, device="cuda")
+    for c in range(0, plan.k, 32):
+        s = G1[:, c:c + 32].abs().amax(1) / 7 * (1 + 2.0 ** -7)  # a bfloat16 number not below the seventh
+        bound += 0.5 * s[:, None] * G2[:, c:c + 32].sum(1)[None, :]
+    return bound.cpu().numpy()
+
+
+def test_gallery_scores():
+    import torch
+
+    from hyperion_amd.gallery import PLDAGallery
+
+    m, plda = _model()
+    x = synth.sample_splda(m, 40, 6, seed=7)
+    xe, xt = x[::2], x[1::2][:33]
+    g = PLDAGallery(plda).enrol(xe)
+    want = plda.llr_1vs1(xe, xt)
+    got = g.llr(xt)
+    assert isinstance(got, np.ndarray) and got.shape == want.shape and got.dtype == want.dtype
+    bound = _bound(g.plan, xe, xt) + 1e-4 * np.maximum(np.abs(want), 1)
+    assert (np.abs(got - want) <= bound).all()
+    # a rounding to 15 levels moves a score by a fraction of what scores differ by
+    assert np.std(got - want) <= 0.2 * np.std(want)
+    dev = g.llr(torch.from_numpy(xt).cuda())
+    assert dev.is_cuda and np.abs(dev.cpu().numpy() - got).max() <= 1e-5 * np.abs(got).max()
+    rows, best = g.identify(xt, 3)
+    assert rows.shape == best.shape == (33, 3)
+    assert np.allclose(np.take_along_axis(got.T, rows, 1), best, rtol=1e-6, atol=1e-6)
+    assert np.allclose(best, -np.sort(-got.T, axis=1)[:, :3], rtol=1e-6, atol=1e-6)
+    spk = np.repeat(np.arange(40), 6)
+    assert (spk[::2][rows[:, 0]] == spk[1::2][:33]).mean() >= (spk[::2][want.argmax(0)] == spk[1::2][:33]).mean() - 0.1
+
+
+def test_gallery_partitions():
+    from hyperion_amd.gallery import PLDAGallery
+
+    m, plda = _model()
+    x = synth.sample_splda(m, 60, 4, seed=9)
+    rng = np.random.RandomState(1)
+    xe, xt = x[:200], x[200:]
+    pe, pt = rng.choice([0, 1, 3], 200, p=[0.6, 0.39, 0.01]), rng.choice([0, 2, 3], 40)
+    g = PLDAGallery(plda).enrol(xe, pe, 4)
+    whole = PLDAGallery(plda).enrol(xe).llr(xt)
+    blocks = g.llr(xt, pt)
+    assert len(blocks) == 4
+    for e, (rows, tests, s) in enumerate(blocks):
+        assert np.array_equal(rows, np.where(pe == e)[0]) and np.array_equal(tests, np.where(pt == e)[0])
+        assert s.shape == (len(rows), len(tests)) and np.array_equal(s, whole[np.ix_(rows, tests)])
+    rows, best = g.identify(xt, 5, pt)
+    for i in range(40):
+        mine = np.where(pe == pt[i])[0]
+        k = min(5, len(mine))
+        assert (rows[i, k:] == -1).all() and np.isneginf(best[i, k:]).all()
+        assert np.array_equal(best[i, :k], -np.sort(-whole[mine, i])[:k]) and set(rows[i, :k]) <= set(mine)
+    with pytest.raises(ValueError, match="4 partitions"):
+        g.llr(xt)
+    with pytest.raises(ValueError, match="lie in"):
+        g.llr(xt, pt + 1)
+    with pytest.raises(ValueError, match="partition numbers"):
+        g.identify(xt, 5, pt[:-1])
+
+
+def test_gallery_rows_that_are_not_finite_are_never_named():
+    from hyperion_amd.gallery import PLDAGallery
+
+    m, plda = _model()
+    x = synth.sample_splda(m, 10, 4, seed=11)
+    x[3, 5] = np.nan
+    g = PLDAGallery(plda).enrol(x[:20])
+    assert np.isnan(g.llr(x[20:])[3]).all()
+    rows, best = g.identify(x[20:], 20)
+    assert not (rows == 3).any() and (rows[:, -1] == -1).all() and np.isneginf(best[:, -1]).all()
+    assert PLDAGallery(plda).enrol(x[:20]).identify(x[:0], 2)[0].shape == (0, 2)
+    with pytest.raises(ValueError, match="nothing is enrolled"):
+        PLDAGallery(plda).llr(x)
+    with pytest.raises(ValueError, match="at least 1"):
+        g.identify(x, 0)
+
+
+def test_packing_by_group():
+    """Rows packed with the maps of their group are the rows packed group by group (hypmi_book_pack)."""
+    import torch
+
+    from hyperion_amd import engine
+
+    rng = np.random.RandomState(3)
+    sizes, K = [5, 0, 70, 1], 33
+    s = torch.from_numpy(rng.randn(76, K)).float().cuda()
+    maps, c = rng.randn(4, 4, K).astype(np.float32), rng.randn(4).astype(np.float32)
+    G1, G2 = engine.grouped_pack(s, engine.RowGroups(sizes), maps, c)
+    e = np.repeat(np.arange(4), sizes)
+    v, w = s.double().cpu().numpy(), maps.astype(float)[e]
+    g, h = (v + w[:, 0]) * w[:, 1], (v + w[:, 2]) * w[:, 3]
+    q = 0.5 * ((g * g).sum(1) - (h * h).sum(1))
+    # two roundings each of g and h, K of the sum of |g^2| + |h^2|
+    tol = 2.0 ** -24 * (K + 8) * ((g * g).sum(1) + (h * h).sum(1))
+    for G, at_q, add in ((G1, K, 0), (G2, K + 1, c[e])):
+        G = G.double().cpu().numpy()
+        assert np.abs(G[:, :K] - g).max() <= 2.0 ** -22 * np.abs(w[:, 1]).max() * (np.abs(v).max() + np.abs(w).max())
+        assert (np.abs(G[:, at_q] - (q + add)) <= tol + 2.0 ** -23 * np.abs(q + add)).all()
+        assert (G[:, 2 * K + 1 - at_q] == 1).all() and (G[:, K + 2:] == 0).all()
+    assert torch.equal(engine.grouped_pack(s, engine.RowGroups(sizes), maps, c, "enrol")[0], G1)
+    none, only = engine.grouped_pack(s, engine.RowGroups(sizes), maps, c, "test")
+    assert none is None and torch.equal(only, G2)
+    for args, match in (((s, engine.RowGroups(sizes), maps[:3], c), "maps must"), ((s, engine.RowGroups(sizes), maps, c, "x"), "sides"),
+                        ((s[:5], engine.RowGroups(sizes), maps, c), "has 5 rows")):
+        with pytest.raises(ValueError, match=match):
+            engine.grouped_pack(*args)
