@@ -196,6 +196,7 @@ SIGNATURES = {
     "hypmi_grouped_score": (ctypes.c_int, [c_void_p, i64, c_void_p, i64, ctypes.c_int, c_void_p, c_void_p, c_void_p,
                                            c_void_p, ctypes.c_int, i64, c_void_p, c_void_p]),
     "hypmi_grouped_gram_span": (ctypes.c_int, []),
+    "hypmi_grouped_gram_split": (ctypes.c_int, []),
     "hypmi_grouped_gram_workspace_bytes": (i64, [i64, ctypes.c_int]),
     "hypmi_grouped_gram_f64": (ctypes.c_int, [c_void_p, ctypes.c_int, i64, ctypes.c_int, c_void_p, c_void_p, c_void_p,
                                               c_void_p, ctypes.c_int, i64, i64, c_void_p, c_void_p, c_void_p,

@@ -10,8 +10,11 @@
 // sixteen before them are multiplied.  Only blocks on or above the diagonal are computed (and three quarters of
 // those on it), and both halves are written from them.
 //
-// A group with more than `span` rows is cut into chunks; every chunk writes its block to a slot of the
-// workspace and a second kernel adds the slots in chunk order, so results do not depend on scheduling.
+// Groups differ in size by orders of magnitude, and a wave with a thousand rows runs for 25 us: a chunk of more than
+// GRAM_SPLIT rows is therefore shared by the four waves of a workgroup, a quarter each, which add their blocks in
+// shared memory; in smaller ones every wave has a block of its own.  A group of more than GRAM_SPAN rows is cut into
+// chunks; every chunk writes its block to a slot of the workspace and a second kernel adds the slots in chunk order.
+// No sum depends on scheduling.
 #include "grouped.h"
 
 #include <type_traits>
@@ -24,10 +27,10 @@ struct GramArgs {
     int d;
     const double* w;
     const int64_t* offsets;
-    const int64_t* chunks;  // [n_groups + 1] prefix of max(1, ceil(size / GRAM_SPAN))
-    const int64_t* slots;   // [n_groups + 1] the same for groups of several chunks, 0 for the others
+    const int64_t* units;   // [n_groups + 1] prefix of the units of work: four for a shared chunk, one for a small one
+    const int64_t* slots;   // [n_groups + 1] prefix of the number of chunks of groups that have several, 0 for the others
     int n_groups;
-    int64_t n_chunks;
+    int64_t n_units;
     const int32_t* order;
     double* C;
     double* F;
@@ -36,7 +39,8 @@ struct GramArgs {
     int nb, pairs;
 };
 
-constexpr int GRAM_SPAN = 1024;  // rows of one chunk
+constexpr int GRAM_SPAN = 4096;  // rows of one chunk
+constexpr int GRAM_SPLIT = 192;  // a chunk of more rows is shared by four waves
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -60,19 +64,32 @@ struct GramBatch {
 template <typename XT, bool ORDERED, bool WEIGHTED>
 __global__ __launch_bounds__(256, 2) void grouped_gram_kernel(GramArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
+    // [wave][tile][16][17] while a chunk's blocks are added up, the first 16 x 17 of a wave's part to turn a tile
+    __shared__ double sums[4][4][16][17];
+    __shared__ double sums_f[4][2][16];
     const int quads = (g.pairs + 3) >> 2;
-    const int64_t t = xcd_slot(blockIdx.x, g.n_chunks * quads);
+    const int64_t t = xcd_slot(blockIdx.x, g.n_units * quads);
     if (t < 0) return;
-    const int64_t chunk = t / quads;
-    const int pair = (int)(t - chunk * quads) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (pair >= g.pairs) return;
-    const int e = find_group(g.chunks, g.n_groups, chunk);
-    const int64_t ch = chunk - g.chunks[e];
-    const int64_t s_beg = g.offsets[e] + ch * GRAM_SPAN;
-    const int64_t s_lim = g.offsets[e + 1];
-    const int ns = s_lim - s_beg < GRAM_SPAN ? (int)(s_lim - s_beg) : GRAM_SPAN;
+    const int64_t unit = t / quads;
+    const int quad = (int)(t - unit * quads);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int e = find_group(g.units, g.n_groups, unit);
+    const int64_t u0 = unit - g.units[e], s_lim = g.offsets[e + 1], size = s_lim - g.offsets[e];
+    // whole chunks have four units each, so that the remainder starts at a multiple of four
+    const int64_t ch = u0 >> 2;
+    int64_t s_beg = g.offsets[e] + ch * GRAM_SPAN;
+    int ns = s_lim - s_beg < GRAM_SPAN ? (int)(s_lim - s_beg) : GRAM_SPAN;
+    const bool split = ns > GRAM_SPLIT;
+    const int pair = quad * 4 + (split ? (int)(u0 & 3) : wave);
+    if (pair >= g.pairs) return;  // the whole workgroup where the chunk is shared
     int bi, bj;
     pair_of(pair, g.nb, bi, bj);
+    if (split) {
+        const int part = ((ns + 63) >> 6) << 4;  // a quarter, in batches of sixteen
+        const int from = wave * part < ns ? wave * part : ns;
+        ns = ns - from < part ? ns - from : part;
+        s_beg += from;
+    }
     const bool diag = bi == bj;
     const int lane = threadIdx.x & 63, l15 = lane & 15, l4 = lane >> 4;
     const XT* X = static_cast<const XT*>(g.x);
@@ -170,32 +187,69 @@ __global__ __launch_bounds__(256, 2) void grouped_gram_kernel(GramArgs g) {
         f[h] += __shfl_xor(f[h], 16);
         f[h] += __shfl_xor(f[h], 32);
     }
-    const int64_t slot = g.slots[e + 1] > g.slots[e] ? g.slots[e] + ch : -1;
+    const int64_t slot = size > GRAM_SPAN ? g.slots[e] + ch : -1;
     double* part = g.part + (slot * g.pairs + pair) * 1024;
     double* C = g.C + (int64_t)e * g.d * g.d;
+    // tile (i, j) of the block, lane: rows l4 + 4 q, column l15
+    auto write = [&](int i, int j, const f64x4& v) {
+        const int r0 = 32 * bi + 16 * i, c0 = 32 * bj + 16 * j;
+        if (slot >= 0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[(16 * i + l4 + 4 * q) * 32 + 16 * j + l15] = v[q];
+            return;
+        }
+        double(*turn)[17] = sums[wave][split ? i * 2 + j : 0];  // this wave's own until the end
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = r0 + l4 + 4 * q, c = c0 + l15;
+            if (r <= c && c < g.d) C[(int64_t)r * g.d + c] = v[q];
+            turn[l15][l4 + 4 * q] = v[q];
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // the other half: rows of the transposed tile
+            const int c = c0 + l4 + 4 * q, r = r0 + l15;
+            if (r < c && c < g.d) C[(int64_t)c * g.d + r] = turn[l4 + 4 * q][l15];
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto write_f = [&](double v, int h) {  // 16 lanes: feature 32 bi + 16 h + l15
+        const int c = 32 * bi + 16 * h + l15;
+        if (slot >= 0) g.part_f[slot * 32 * g.nb + c] = v;
+        else if (c < g.d) g.F[(int64_t)e * g.d + c] = v;
+    };
+    if (split) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sums[wave][i * 2 + j][l4 + 4 * q][l15] = acc[i][j][q];
+        if (diag && l4 < 2) sums_f[wave][l4][l15] = l4 ? f[1] : f[0];
+        __syncthreads();
+        f64x4 v;  // wave w finishes tile w
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            v[q] = sums[0][wave][l4 + 4 * q][l15];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) v[q] += sums[w][wave][l4 + 4 * q][l15];
+        }
+        double fs = 0.0;
+        if (diag && wave < 2 && l4 == 0) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) fs += sums_f[w][wave][l15];
+        }
+        __syncthreads();  // `write` turns tiles in the same memory
+        if (!diag || wave != 2) write(wave >> 1, wave & 1, v);
+        if (diag && wave < 2 && l4 == 0) write_f(fs, wave);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int rr = 16 * i + l4 + 4 * q, cc = 16 * j + l15;
-                if (slot >= 0) {
-                    part[rr * 32 + cc] = acc[i][j][q];
-                } else {
-                    const int r = 32 * bi + rr, c = 32 * bj + cc;
-                    if (r <= c && c < g.d) {
-                        C[(int64_t)r * g.d + c] = acc[i][j][q];
-                        if (r < c) C[(int64_t)c * g.d + r] = acc[i][j][q];
-                    }
-                }
-            }
-    if (diag && l4 < 2) {
-        const int c = 32 * bi + 16 * l4 + l15;
-        const double v = l4 ? f[1] : f[0];
-        if (slot >= 0) g.part_f[slot * 32 * g.nb + c] = v;
-        else if (c < g.d) g.F[(int64_t)e * g.d + c] = v;
-    }
+            if (i <= j || !diag) write(i, j, acc[i][j]);
+    if (diag && l4 < 2) write_f(l4 ? f[1] : f[0], l4);
 #endif
 }
 
@@ -234,6 +288,7 @@ __global__ __launch_bounds__(256) void grouped_gram_reduce_kernel(GramArgs g) {
 using namespace hypmi_detail;
 
 extern "C" int hypmi_grouped_gram_span(void) { return GRAM_SPAN; }
+extern "C" int hypmi_grouped_gram_split(void) { return GRAM_SPLIT; }
 
 extern "C" int64_t hypmi_grouped_gram_workspace_bytes(int64_t n_slots, int d) {
     if (n_slots <= 0 || d <= 0) return 0;
@@ -242,25 +297,25 @@ extern "C" int64_t hypmi_grouped_gram_workspace_bytes(int64_t n_slots, int d) {
 }
 
 extern "C" int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, int d, const double* w,
-                                      const int64_t* offsets, const int64_t* chunks, const int64_t* slots,
-                                      int n_groups, int64_t n_chunks, int64_t n_slots, const int32_t* order, double* C,
+                                      const int64_t* offsets, const int64_t* units, const int64_t* slots,
+                                      int n_groups, int64_t n_units, int64_t n_slots, const int32_t* order, double* C,
                                       double* F, void* workspace, int64_t workspace_bytes, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    HYPMI_REQUIRE(n_groups >= 0 && n_chunks >= 0 && n_slots >= 0 && d > 0, "grouped_gram: bad shape");
+    HYPMI_REQUIRE(n_groups >= 0 && n_units >= 0 && n_slots >= 0 && d > 0, "grouped_gram: bad shape");
     HYPMI_REQUIRE(x_type == HYPMI_F32 || x_type == HYPMI_F64, "grouped_gram: vectors must be fp32 or fp64");
     HYPMI_REQUIRE(ldx >= d, "grouped_gram: bad leading dimension");
     if (n_groups == 0) return HYPMI_OK;
-    HYPMI_REQUIRE(offsets && chunks && slots && C && F, "grouped_gram: null pointer");
-    HYPMI_REQUIRE(n_chunks >= n_groups, "grouped_gram: every group has a chunk");
+    HYPMI_REQUIRE(offsets && units && slots && C && F, "grouped_gram: null pointer");
+    HYPMI_REQUIRE(n_units >= n_groups, "grouped_gram: every group has a unit of work");
     HYPMI_REQUIRE(workspace_bytes >= hypmi_grouped_gram_workspace_bytes(n_slots, d) && (n_slots == 0 || workspace),
                   "grouped_gram: workspace too small");
     const int nb = (d + 31) / 32;
     HYPMI_REQUIRE(nb <= 2048, "grouped_gram: more than 65536 features");
     const int pairs = nb * (nb + 1) / 2;
     double* part = static_cast<double*>(workspace);
-    const GramArgs g = {x, ldx, d, w, offsets, chunks, slots, n_groups, n_chunks, order, C, F, part,
+    const GramArgs g = {x, ldx, d, w, offsets, units, slots, n_groups, n_units, order, C, F, part,
                         part ? part + n_slots * pairs * 1024 : nullptr, nb, pairs};
-    const int64_t grid = xcd_grid(n_chunks * ((pairs + 3) / 4));
+    const int64_t grid = xcd_grid(n_units * ((pairs + 3) / 4));
     const int64_t reduce = n_slots ? (int64_t)n_groups * pairs : 0;
     HYPMI_REQUIRE(grid <= 0x7fffffffLL && reduce <= 0x7fffffffLL, "grouped_gram: too many workgroups");
     const dim3 blocks((unsigned)grid), threads(256);

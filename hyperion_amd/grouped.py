@@ -92,15 +92,16 @@ class RowGroups(_Plan):
         if order is not None:
             self._set_order(order)
         lib = _lib.load()
-        span = lib.hypmi_grouped_gram_span()
-        cut = _ceil(sizes, span)
+        span, split = lib.hypmi_grouped_gram_span(), lib.hypmi_grouped_gram_split()
+        cut, rest = _ceil(sizes, span), sizes % span
         prefix = [_prefix(_ceil(sizes, t)) for t in _AFFINE_TILES]
-        chunks, slots = _prefix(np.maximum(cut, 1)), _prefix(np.where(cut > 1, cut, 0))
-        self._tab = _tables([self.offsets] + prefix + [chunks, slots], self.device)
+        units = _prefix(4 * (sizes // span) + np.where(rest > split, 4, (rest > 0) | (sizes == 0)))
+        slots = _prefix(np.where(cut > 1, cut, 0))
+        self._tab = _tables([self.offsets] + prefix + [units, slots], self.device)
         base = self._tab.data_ptr()
         self._rows = [base + 8 * i * (self.num_groups + 1) for i in range(6)]  # device pointers of the tables
         self._n_tiles = dict(zip(_AFFINE_TILES, (int(p[-1]) for p in prefix)))
-        self._n_chunks, self._n_slots = int(chunks[-1]), int(slots[-1])
+        self._n_units, self._n_slots = int(units[-1]), int(slots[-1])
         self._order_ptr = None if self.order is None else self.order.data_ptr()
         # rows per workgroup of the affine map: the largest tile that most rows can fill
         used = int(np.count_nonzero(sizes))
@@ -409,7 +410,7 @@ def grouped_gram64(x, groups, w=None):
     ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
     if E:
         _run(lib.hypmi_grouped_gram_f64, x.device, (groups,), x.data_ptr(), kinds[x.dtype], ldx, d,
-             None if w is None else w.data_ptr(), groups._rows[0], groups._rows[4], groups._rows[5], E, groups._n_chunks,
+             None if w is None else w.data_ptr(), groups._rows[0], groups._rows[4], groups._rows[5], E, groups._n_units,
              groups._n_slots, groups._order_ptr, C.data_ptr(), F.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return C, F
 

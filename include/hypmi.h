@@ -577,13 +577,16 @@ int hypmi_grouped_score(const float* G1, int64_t ld1, const float* G2, int64_t l
 
 /* C_e = sum_r w_r x_r x_r^T [d x d] and F_e = sum_r w_r x_r [d] over the rows of every group, in float64 (w NULL:
  * 1; indexed by row of x).  x: HYPMI_F32 or HYPMI_F64.  C [n_groups x d x d] is exactly symmetric, empty groups
- * are zero, and the sums are added in a fixed order (same bits from run to run).  chunks: prefix sums of
- * max(1, ceil(size / hypmi_grouped_gram_span())); slots: the same with 0 in place of 1.  workspace:
- * hypmi_grouped_gram_workspace_bytes(n_slots, d) bytes, 8-byte aligned. */
+ * are zero, and the sums are added in a fixed order (same bits from run to run).  A group is cut into chunks of
+ * hypmi_grouped_gram_span() rows; a chunk of more than hypmi_grouped_gram_split() rows counts four units, a smaller
+ * one (and that of an empty group) one.  units: prefix sums of the groups' units; slots: prefix sums of the number of
+ * chunks of the groups that have several, 0 for the others.  workspace: hypmi_grouped_gram_workspace_bytes(n_slots, d)
+ * bytes, 8-byte aligned. */
 int hypmi_grouped_gram_span(void);
+int hypmi_grouped_gram_split(void);
 int64_t hypmi_grouped_gram_workspace_bytes(int64_t n_slots, int d);
 int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, int d, const double* w, const int64_t* offsets,
-                           const int64_t* chunks, const int64_t* slots, int n_groups, int64_t n_chunks,
+                           const int64_t* units, const int64_t* slots, int n_groups, int64_t n_units,
                            int64_t n_slots, const int32_t* order, double* C, double* F, void* workspace,
                            int64_t workspace_bytes, void* stream);
 

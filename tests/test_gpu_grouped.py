@@ -314,6 +314,8 @@ GRAM = [
     ([100, 41], 200),
     ([64], 520),
     ([0, 0], 9),
+    ([192, 193, 256, 4095], 50),
+    ([4096, 4097, 4289, 0, 8192], 20),
 ]
 
 

@@ -67,7 +67,7 @@ def test_refusals_of_the_c_abi():
     assert lib.hypmi_grouped_gram_f64(P, 0, 8, 8, None, P, P, P, 1, 1, 2, None, P, P, P, 100, None) == -1
     assert b"workspace" in lib.hypmi_last_error()
     assert lib.hypmi_grouped_gram_f64(P, 0, 8, 8, None, P, P, P, 2, 1, 0, None, P, P, None, 0, None) == -1
-    assert b"chunk" in lib.hypmi_last_error()
+    assert b"unit of work" in lib.hypmi_last_error()
 
     assert "coordinates" in _refused("hypmi_q4_rows", P, 600, 513, P, P, 1, 1, P, P, P, None)
     assert "bad shape" in _refused("hypmi_q4_rows", P, 30, 30, P, P, 1, 1, P, P, P, None)
