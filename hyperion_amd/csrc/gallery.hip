@@ -27,6 +27,7 @@ namespace hypmi_detail {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+constexpr int Q4_RUN = 8;        // tasks dealt to an XCD at a time
 constexpr int Q4_BLOCK = 64;     // rows of a block
 
 // One thread per (row slot, k-step).
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256, TT == 4 ? 2 : 3) void q4_score_kernel(Q4Args g
     __shared__ __attribute__((aligned(16))) int up_s[16 * TT];
     __shared__ __attribute__((aligned(16))) float add_s[16 * TT];
 
-    const int64_t t = xcd_slot(blockIdx.x, g.n_tasks);
+    const int64_t t = xcd_task(blockIdx.x, g.n_tasks, Q4_RUN);
     if (t < 0) return;
     const int e = find_group(g.tasks, g.n_groups, t);
     const int64_t n = g.off_g[e + 1] - g.off_g[e], m_all = g.off_t[e + 1] - g.off_t[e];
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256, TT == 4 ? 2 : 3) void q4_score_kernel(Q4Args g
 
 template <int KH, int TT>
 int launch_q4(const Q4Args& g, hipStream_t stream) {
-    const int64_t grid = xcd_grid(g.n_tasks);
+    const int64_t grid = xcd_grid(g.n_tasks, Q4_RUN);
     HYPMI_REQUIRE(grid <= 0x7fffffffLL, "q4_score: too many workgroups");
     const int lds = TT * KH * g.phases * 2048;
     if (lds > 48 * 1024)

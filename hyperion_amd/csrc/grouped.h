@@ -28,16 +28,15 @@ __device__ __forceinline__ int find_group(const int64_t* __restrict__ prefix, in
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// Workgroups are handed to the eight XCDs round robin (a placement assumed for speed only); launch slot b
-// takes entry b / 8 of the eighth that belongs to its XCD, so that neighbouring tiles -- which read the same
-// group's operands -- meet in one L2.  Returns -1 for the slots that pad the grid.
-__device__ __forceinline__ int64_t xcd_slot(int64_t b, int64_t n) {
-    const int64_t per = (n + 7) >> 3;
-    const int64_t t = (b & 7) * per + (b >> 3);
-    return (b >> 3) < per && t < n ? t : -1;
+// Workgroups are handed to the eight XCDs round robin (a placement assumed for speed only).  Runs of `run` tasks are
+// dealt to the XCDs in turn: neighbouring tasks, which read the same operands, meet in one L2, and tasks of unequal
+// cost, which also stand together, do not end up on one XCD.  Returns -1 for the slots that pad the grid.
+__device__ __forceinline__ int64_t xcd_task(int64_t b, int64_t n, int run) {
+    const int64_t k = b >> 3, t = ((k / run) * 8 + (b & 7)) * run + k % run;
+    return t < n ? t : -1;
 }
 
-inline int64_t xcd_grid(int64_t n) { return (n + 7) / 8 * 8; }
+inline int64_t xcd_grid(int64_t n, int run) { return (n + 8 * run - 1) / (8 * run) * (8 * run); }
 
 // 2^e as a float, -126 <= e <= 127
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }

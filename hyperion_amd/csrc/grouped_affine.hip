@@ -51,6 +51,8 @@ struct Load4<__bf16> {
     }
 };
 
+constexpr int AFFINE_RUN = 8;  // tiles dealt to an XCD at a time
+
 struct AffineArgs {
     const void* x;
     int64_t ldx;
@@ -94,7 +96,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     __shared__ int rows[TM];
     __shared__ float norm[CW][TM];
 
-    const int64_t t = xcd_slot(blockIdx.x, g.n_tiles);
+    const int64_t t = xcd_task(blockIdx.x, g.n_tiles, AFFINE_RUN);
     if (t < 0) return;
     const int e = find_group(g.tiles, g.n_groups, t);
     const int64_t r0 = g.offsets[e] + (t - g.tiles[e]) * TM;
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(256) void grouped_pack_kernel(const float* __restri
 template <typename XT, int RT>
 int launch_affine(const AffineArgs& g, hipStream_t stream) {
     const int per = 16;  // column tiles of a workgroup
-    const int64_t gx = xcd_grid(g.n_tiles), gy = (g.ct + per - 1) / per;
+    const int64_t gx = xcd_grid(g.n_tiles, AFFINE_RUN), gy = (g.ct + per - 1) / per;
     HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
     hipLaunchKernelGGL((grouped_affine_kernel<XT, RT>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, stream, g);
     HYPMI_HIP(hipGetLastError());

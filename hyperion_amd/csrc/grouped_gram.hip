@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void grouped_gram_kernel(GramArgs g) {
     __shared__ double sums[4][4][16][17];
     __shared__ double sums_f[4][2][16];
     const int quads = (g.pairs + 3) >> 2;
-    const int64_t t = xcd_slot(blockIdx.x, g.n_units * quads);
+    const int64_t t = xcd_task(blockIdx.x, g.n_units * quads, quads);
     if (t < 0) return;
     const int64_t unit = t / quads;
     const int quad = (int)(t - unit * quads);
@@ -315,7 +315,7 @@ extern "C" int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, in
     double* part = static_cast<double*>(workspace);
     const GramArgs g = {x, ldx, d, w, offsets, units, slots, n_groups, n_units, order, C, F, part,
                         part ? part + n_slots * pairs * 1024 : nullptr, nb, pairs};
-    const int64_t grid = xcd_grid(n_units * ((pairs + 3) / 4));
+    const int64_t grid = xcd_grid(n_units * ((pairs + 3) / 4), (pairs + 3) / 4);
     const int64_t reduce = n_slots ? (int64_t)n_groups * pairs : 0;
     HYPMI_REQUIRE(grid <= 0x7fffffffLL && reduce <= 0x7fffffffLL, "grouped_gram: too many workgroups");
     const dim3 blocks((unsigned)grid), threads(256);

@@ -34,6 +34,7 @@ struct ScoreArgs {
     float* S;
 };
 
+constexpr int SCORE_RUN = 8;     // tasks dealt to an XCD at a time
 constexpr int SCORE_SPAN = 512;  // test rows one workgroup walks at most
 
 template <int KS, int RT>  // k-steps of 32 coordinates, row tiles of 16 per wave
@@ -43,7 +44,7 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
     __shared__ uint4 tile[2][2 * KS * 2 * 64];  // [buffer][(column tile, k-step, part, lane)]
     __shared__ int scale[2][32];
 
-    const int64_t t = xcd_slot(blockIdx.x, g.n_tasks);
+    const int64_t t = xcd_task(blockIdx.x, g.n_tasks, SCORE_RUN);
     if (t < 0) return;
     const int e = find_group(g.tasks, g.n_groups, t);
     const int64_t n1 = g.off1[e + 1] - g.off1[e], n2 = g.off2[e + 1] - g.off2[e];
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
 template <int KS>
 int launch_score(const ScoreArgs& g, hipStream_t stream) {
     constexpr int RT = KS <= 6 ? 2 : 1;
-    const int64_t grid = xcd_grid(g.n_tasks);
+    const int64_t grid = xcd_grid(g.n_tasks, SCORE_RUN);
     HYPMI_REQUIRE(grid <= 0x7fffffffLL, "grouped_score: too many workgroups");
     hipLaunchKernelGGL((grouped_score_kernel<KS, RT>), dim3((unsigned)grid), dim3(256), 0, stream, g);
     HYPMI_HIP(hipGetLastError());
