@@ -73,7 +73,8 @@ struct AffineArgs {
 };
 
 // RT row tiles of 16 per workgroup of eight waves, which take two column tiles of 16 each.  Coordinates are taken in
-// chunks of 256 / RT, so that every thread holds eight values of a chunk whatever RT is; the chunk at hand sits in
+// chunks: 32 for RT = 8, where many workgroups follow one another, up to 1024 / RT for the small tiles, where a row is
+// usually one chunk and everything it needs is requested at once.  The chunk at hand sits in
 // LDS as pairs in operand order (lane l of a 16 x 32 tile: row l & 15, coordinates 8 (l >> 4) .. + 7; the row is
 // XORed with 4 (l >> 4) so that the four coordinate groups of a row fall into different banks when they are written),
 // the next one is on its way in registers.  Memory operations of a wave complete in order, so the weights of a whole
@@ -83,14 +84,15 @@ template <typename XT, int RT>
 __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(AffineArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int TM = 16 * RT;
-    constexpr int KC = 256 / RT;
+    constexpr int KC = RT == 8 ? 32 : 1024 / RT;
     constexpr int NP = sizeof(XT) == 4 ? 2 : 1;  // parts of x
-    constexpr int LPR = RT == 1 ? 32 : 64 / RT;  // lanes that load one row
-    constexpr int RPT = RT == 1 ? 1 : 2;         // rows per thread
-    constexpr int F4 = 2 / RPT;                  // groups of four coordinates per thread and row
+    constexpr int LPR = RT == 1 ? 32 : 8;        // lanes that load one row
+    constexpr int RPT = TM * LPR / 512;          // rows per thread
+    constexpr int F4 = KC / (4 * LPR);           // groups of four coordinates per thread and row
     constexpr int CW = 8, NT = 2;
     constexpr int KSC = KC / 32;                 // k-steps per chunk
-    __shared__ uint4 tile[2][KSC * RT * NP * 64];
+    extern __shared__ __attribute__((aligned(16))) uint4 tile_mem[];  // two buffers, one where a row is one chunk
+    constexpr int BUF = KSC * RT * NP * 64;
     __shared__ int exps[3][TM];  // a chunk's scales are still read while those of the next but one are written
     __shared__ int lowered[2];  // the chunk for which a scale was lowered last, by buffer
     __shared__ int rows[TM];
@@ -141,8 +143,8 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
             for (int f = 0; f < F4; ++f)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(v[i][f][q]));
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            m = dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(m)));
+            if (LPR == 32) m = swap16_max(dpp_max<0x140>(m));
             const int ex = __builtin_amdgcn_frexp_expf(m);
             if (m > 0.f && ex + run[i] > 15) {
                 run[i] = 9 - ex;
@@ -155,11 +157,12 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
 #pragma unroll
             for (int f = 0; f < F4; ++f) {
                 const int k = 4 * (c + LPR * f);  // inside the chunk
+                if (F4 > 1 && ch * KC + 4 * LPR * f >= 32 * g.ks) break;
                 const int s = k >> 5, kq = (k >> 3) & 3, half = (k >> 2) & 1;
                 f16x4 x0, x1;
                 split_pair4(v[i][f], up, x0, x1);
                 f16x4* dst = reinterpret_cast<f16x4*>(
-                                 &tile[buf][((s * RT + rt) * NP) * 64 + kq * 16 + (r16 ^ (4 * kq))]) + half;
+                                 &tile_mem[buf * BUF + ((s * RT + rt) * NP) * 64 + kq * 16 + (r16 ^ (4 * kq))]) + half;
                 dst[0] = x0;
                 if (NP == 2) dst[2 * 64] = x1;
             }
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     // the chunk loop of a wave with `tiles` column tiles
     auto walk = [&](auto tiles_tag) {
         constexpr int N = decltype(tiles_tag)::value;
-        constexpr int WS = KSC < 4 ? KSC : 4;  // k-steps of weights in registers
+        constexpr int WS = RT == 8 ? 1 : RT == 4 ? 2 : 4;  // k-steps of weights in registers
         const uint4* w0p = wp + ((int64_t)e * g.ct + ct0) * w_tile;
         const uint4* w1p = wp + ((int64_t)e * g.ct + ct1) * w_tile;
         f16x8 w[WS][N > 0 ? N : 1][2];
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
         auto step = [&](int buf, int slot, int s) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                const uint4* xp = &tile[buf][((s * RT + i) * NP) * 64 + xs];
+                const uint4* xp = &tile_mem[buf * BUF + ((s * RT + i) * NP) * 64 + xs];
                 const f16x8 x0 = __builtin_bit_cast(f16x8, xp[0]);
 #pragma unroll
                 for (int j = 0; j < N; ++j)
@@ -236,12 +239,12 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
                             for (int q = 0; q < 4; ++q) acc[i][j][q] = ldexpf(acc[i][j][q], by);
                     }
                 }
-                if constexpr (KSC <= 4) {
+                if constexpr (KSC == WS) {
 #pragma unroll
                     for (int s = 0; s < KSC; ++s)
                         if (ch * KSC + s < g.ks) step(buf, s, s);
                 } else {
-                    // a long chunk of few rows: the weights go round a ring of four k-steps
+                    // a long chunk: the weights go round a ring of WS k-steps
                     for (int s0 = 0; s0 < KSC; s0 += WS) {
                         if (ch * KSC + s0 >= g.ks) break;
 #pragma unroll
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
             }
             if (ch + 1 < chunks) {
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (KSC <= 4) {
+                if constexpr (KSC == WS) {
 #pragma unroll
                     for (int s = 0; s < KSC; ++s) weights(s, (ch + 1) * KSC + s);
                 }
@@ -428,7 +431,12 @@ int launch_affine(const AffineArgs& g, hipStream_t stream) {
     const int per = 16;  // column tiles of a workgroup
     const int64_t gx = xcd_grid(g.n_tiles, AFFINE_RUN), gy = (g.ct + per - 1) / per;
     HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
-    hipLaunchKernelGGL((grouped_affine_kernel<XT, RT>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, stream, g);
+    constexpr int KC = RT == 8 ? 32 : 1024 / RT;
+    const int lds = (g.d_in > KC ? 2 : 1) * KC * 16 * RT * (sizeof(XT) == 4 ? 4 : 2);
+    if (lds > 48 * 1024)
+        HYPMI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&grouped_affine_kernel<XT, RT>),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL((grouped_affine_kernel<XT, RT>), dim3((unsigned)gx, (unsigned)gy), dim3(512), lds, stream, g);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
 }

@@ -90,6 +90,12 @@ AFFINE = [
     ([1500, 1029], 515, 64, True, False),
     ([7, 9], 1024, 512, True, False),
     ([0, 0], 8, 8, True, False),
+    # many rows a group: the kernel whose workgroups take several tiles
+    ([40000, 0, 3000], 64, 20, True, False),
+    ([2500, 1, 2700], 67, 256, True, True),
+    ([1001, 1500], 190, 270, True, False),
+    ([36000], 129, 33, False, True),
+    ([3000, 1300, 2500], 321, 130, True, False),
 ]
 
 
@@ -113,14 +119,15 @@ def test_affine(case, dtype):
     _assert_close(y, want, bound, rms)
 
 
-def test_affine_scales():
+@pytest.mark.parametrize("sizes", [[50, 3, 200], [2, 1, 9], [1300, 1001, 1200]])
+def test_affine_scales(sizes):
     """Rows and columns of very different magnitudes, zero rows, and rows that grow along their coordinates (the
     scale of a row is lowered while it is read)."""
     torch = _torch()
     from hyperion_amd import engine
 
     r = _rng(5)
-    d, m, sizes = 700, 40, [50, 3, 200]
+    d, m = 700, 40
     n = sum(sizes)
     x = r.randn(n, d) * 10.0 ** r.randint(-25, 26, n)[:, None]
     x[::7] = 0
@@ -140,20 +147,22 @@ def test_affine_scales():
     assert fits.mean() > 0.8 and (np.abs(y[over]) >= top * (1 - 1e-3)).all()
 
 
-def test_affine_non_finite_rows_stay_alone():
+@pytest.mark.parametrize("sizes", [[70, 30], [2000, 1200]])
+def test_affine_non_finite_rows_stay_alone(sizes):
     torch = _torch()
     from hyperion_amd import engine
 
     r = _rng(6)
-    x = r.randn(100, 40).astype(np.float32)
+    n = sum(sizes)
+    x = r.randn(n, 70).astype(np.float32)
     clean = torch.from_numpy(x).cuda()
     bad = clean.clone()
-    bad[3, 5], bad[64, 0], bad[99, 39] = float("nan"), float("inf"), -float("inf")
-    bank = engine.AffineBank(r.randn(2, 40, 30))
-    groups = engine.RowGroups([70, 30])
+    bad[3, 5], bad[64, 0], bad[99, 69] = float("nan"), float("inf"), -float("inf")
+    bank = engine.AffineBank(r.randn(2, 70, 30))
+    groups = engine.RowGroups(sizes)
     for lnorm in (False, True):
         a, b = (engine.grouped_affine(t, groups, bank, lnorm=lnorm) for t in (clean, bad))
-        rows = torch.ones(100, dtype=torch.bool)
+        rows = torch.ones(n, dtype=torch.bool)
         rows[[3, 64, 99]] = False
         assert torch.equal(a[rows.cuda()], b[rows.cuda()])
         assert torch.isnan(b[~rows.cuda()]).all()
