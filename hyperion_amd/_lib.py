@@ -188,7 +188,7 @@ SIGNATURES = {
                                              c_void_p, c_void_p]),
     "hypmi_grouped_affine": (ctypes.c_int, [c_void_p, ctypes.c_int, i64, ctypes.c_int, c_void_p, c_void_p,
                                             ctypes.c_int, ctypes.c_int, i64, i64, c_void_p, c_void_p, c_void_p,
-                                            c_void_p, ctypes.c_int, ctypes.c_int, c_void_p, i64, c_void_p]),
+                                            c_void_p, ctypes.c_int, ctypes.c_int, c_void_p, i64, ctypes.c_int, c_void_p]),
     "hypmi_grouped_pack": (ctypes.c_int, [c_void_p, i64, ctypes.c_int, c_void_p, ctypes.c_int, i64, c_void_p, c_void_p,
                                           c_void_p, c_void_p, ctypes.c_int, c_void_p]),
     "hypmi_grouped_score_rows": (ctypes.c_int, [ctypes.c_int]),

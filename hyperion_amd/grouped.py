@@ -5,7 +5,8 @@ block of scores, in one launch.  The names here are part of hyperion_amd.engine.
 A batch is described once, by a RowGroups (sizes on the host, tables on the device) and, for products of
 two sides, a GroupPairs; the operators themselves neither wait for the device nor send it anything, so they
 can be captured in a HIP graph.  Inputs have to be on one device; the work runs on that device's current
-stream."""
+stream.  A RowGroups or GroupPairs can be used on any stream at once; an AffineBank and a Q4Rows are filled by
+launches on the stream they are made on, for which another stream waits as for any tensor."""
 import numpy as np
 
 from . import _lib
@@ -82,6 +83,8 @@ class RowGroups(_Plan):
             raise ValueError("group sizes must not be negative")
         if sizes.size > 0x7fffffff:
             raise ValueError("at most 2^31 - 1 groups")
+        if sizes.sum(dtype=np.float64) > 2.0 ** 40:
+            raise ValueError("at most 2^40 rows")
         self.sizes = sizes
         self.offsets = _prefix(sizes)
         self.num_groups = int(sizes.size)
@@ -136,12 +139,13 @@ class RowGroups(_Plan):
             if lo < 0 or hi > 0x7fffffff:
                 raise ValueError("order must hold row numbers from 0 to 2^31 - 1")
             self.num_rows = hi + 1
-            order = order.to(self.device)
+        # a copy: what the caller does to its tensor later must not reach a launch
+        self.order = torch.empty(self.total, dtype=torch.int32, device=self.device).copy_(order)
+        if self.total:
             seen = torch.zeros(hi + 1, dtype=torch.int8, device=self.device)
-            seen[order.long()] = 1
-            if int(seen.sum(dtype=torch.int64)) != self.total:
+            seen[self.order.long()] = 1
+            if int(seen.sum(dtype=torch.int64)) != self.total:  # waits, for the copy too
                 raise ValueError("order lists a row more than once")
-        self.order = order.to(device=self.device, dtype=torch.int32).contiguous()
 
     def _check(self, x, what):
         if x.get_device() != self.device.index:
@@ -167,6 +171,8 @@ class GroupPairs(_Plan):
         self.rows, self.cols = rows, cols
         self.device = rows.device
         n1, n2 = rows.sizes, cols.sizes
+        if np.sum(n1.astype(np.float64) * n2) > 2.0 ** 52:
+            raise ValueError("at most 2^52 scores")
         self.offsets = _prefix(n1 * n2)
         self.numel = int(self.offsets[-1])
         lib = _lib.load()
@@ -194,13 +200,15 @@ class GroupPairs(_Plan):
     def blocks(self, flat):
         return [self.block(flat, e) for e in range(self.rows.num_groups)]
 
-    def _result(self, out):
+    def _result(self, out, *inputs):
         torch = _torch()
         if out is None:
             return torch.empty(self.numel, dtype=torch.float32, device=self.device)
         if out.dtype != torch.float32 or out.device != self.device or out.dim() != 1 or out.numel() != self.numel \
                 or not out.is_contiguous():
             raise ValueError("out must be a contiguous fp32 vector of %d elements on %s" % (self.numel, self.device))
+        if any(_overlap(a, out) for a in inputs):
+            raise ValueError("out must not share memory with the inputs")
         return out
 
 
@@ -284,7 +292,8 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
     """y_r = x_r W_e + b_e for every row r of group e, with lnorm followed by the length normalisation
     y <- sqrt(dim_e) y / (|y| + 1e-10).  x: device fp32, fp16 or bf16 [n, d_in]; returns device fp32
     [n, d_out] (fp32 accuracy).  With an ordered RowGroups row i of the result belongs to row i of x; rows of
-    no group are zero in a new result and left alone in `out` (fp32, 16-byte aligned rows)."""
+    no group are zero in a new result and left alone in `out` (fp32, 16-byte aligned rows, also a view whose
+    storage goes on behind a row)."""
     torch = _torch()
     kinds = _kinds("affine")
     x, ldx = _device_rows(x, kinds, "x")
@@ -303,11 +312,8 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
     else:
         y = out
         if y.dtype != torch.float32 or y.device != x.device or tuple(y.shape) != (n, d) or \
-                (d > 1 and y.stride(1) != 1) or y.data_ptr() % 16 or (n > 1 and (y.stride(0) % 4 or y.stride(0) < ld)):
-            raise ValueError("out must be fp32 [%d, %d] on %s with 16-byte aligned rows of at least %d elements"
-                             % (n, d, x.device, ld))
-        if n and (y.untyped_storage().nbytes() // 4 - y.storage_offset()) < (n - 1) * y.stride(0) + ld:
-            raise ValueError("the last row of out has no room for %d elements" % ld)
+                (d > 1 and y.stride(1) != 1) or y.data_ptr() % 16 or (n > 1 and (y.stride(0) % 4 or y.stride(0) < d)):
+            raise ValueError("out must be fp32 [%d, %d] on %s with 16-byte aligned rows" % (n, d, x.device))
         if _overlap(x, y):
             raise ValueError("out must not share memory with x")
     tile = groups._affine_tile
@@ -316,7 +322,7 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
         _run(_lib.load().hypmi_grouped_affine, x.device, (groups, bank), x.data_ptr(), kinds[x.dtype], ldx, bank.d_in,
              groups._rows[0], groups._rows[1 + _AFFINE_TILES.index(tile)], tile, groups.num_groups, groups.total, n_tiles,
              groups._order_ptr, bank._w.data_ptr(), bank._c.data_ptr(), bank._dims_ptr, d, int(bool(lnorm)),
-             y.data_ptr(), ld if out is None else (y.stride(0) if n > 1 else ld))
+             y.data_ptr(), ld if out is None else (y.stride(0) if n > 1 else ld), ld if out is None else d)
     return (y if ld == d else y[:, :d]) if out is None else out
 
 
@@ -379,7 +385,7 @@ def grouped_score(G1, G2, pairs, out=None):
     rows = lib.hypmi_grouped_score_rows(kp)
     if not rows:
         raise ValueError("packed width %d has no grouped kernel (multiples of 8 up to 512)" % kp)
-    S = pairs._result(out)
+    S = pairs._result(out, G1, G2)
     i = 1 if rows == 64 else 2
     if pairs.numel:
         _run(lib.hypmi_grouped_score, pairs.device, (pairs, pairs.rows, pairs.cols), G1.data_ptr(), ld1, G2.data_ptr(),
@@ -484,7 +490,7 @@ def q4_score(gallery, G, pairs, out=None):
         buf = _torch().zeros((G.shape[0], ld), dtype=G.dtype, device=G.device)
         buf[:, :k + 2] = G[:, :k + 2]
         G = buf
-    S = pairs._result(out)
+    S = pairs._result(out, G, gallery.codes, gallery.scales, gallery.q)
     if pairs.numel:
         groups = gallery.groups
         _run(_lib.load().hypmi_q4_score, pairs.device, (pairs, pairs.rows, groups, gallery), gallery.codes.data_ptr(),

@@ -72,4 +72,7 @@ class TransformBank(HypModel):
             ids = engine.RowGroups.from_ids(ids, len(self.chains), device=y.device)
         for bank, lnorm in self._banks:
             y = engine.grouped_affine(y, ids, bank, lnorm=lnorm)
+        if not self._banks:  # chains that do nothing
+            ids._check(y, "x")
+            y = y.to(torch.float32, copy=True)
         return y if is_dev else engine.to_host(y, float_cpu())

@@ -548,15 +548,16 @@ int hypmi_grouped_weights(const float* W, const float* b, int n_groups, int d_in
 /* y_r = x_r W_e + b_e for every row r of every group e, and with lnorm != 0 then
  * y_r <- sqrt(dims[e]) y_r / (|y_r| + 1e-10)  (dims NULL: d_out).  x: rows of d_in elements of x_type
  * (HYPMI_F32, HYPMI_F16 or HYPMI_BF16), ldx >= d_in, any alignment of the element type.  y: fp32, 16-byte
- * aligned, ldy a multiple of 4 and at least d_out; columns d_out .. (d_out rounded up to 4) - 1 are set to
- * zero, rows of no group are left as they are.  With `order` row order[i] of x goes to row order[i] of y; no
+ * aligned, ldy a multiple of 4 and at least d_out; cols_y columns of a row are written, d_out or up to the next multiple of 4 (zeros
+ * behind d_out, so that rows which follow one another leave no gaps in the lines that are written); what lies
+ * behind them and rows of no group are left as they are.  With `order` row order[i] of x goes to row order[i] of y; no
  * row may occur twice.  tiles: prefix sums of ceil(size / tile_rows), tile_rows 16, 64 or 128.  Accurate to
  * fp32 (fp16-pair products, fp32 accumulation); a row with a NaN or an infinity comes out
  * without finite values (fp32 rows: as NaN). */
 int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int d_in, const int64_t* offsets,
                          const int64_t* tiles, int tile_rows, int n_groups, int64_t n_rows, int64_t n_tiles,
                          const int32_t* order, const void* weights, const void* columns, const int32_t* dims,
-                         int d_out, int lnorm, float* y, int64_t ldy, void* stream);
+                         int d_out, int lnorm, float* y, int64_t ldy, int cols_y, void* stream);
 
 /* Packed rows of projected rows s [n_rows x lds] by the maps of their group (hypmi_book_pack with maps
  * [n_groups x 4 x K] = shift_t, scale_t, shift_n, scale_n and constants c [n_groups], fp32 on the device; rows in

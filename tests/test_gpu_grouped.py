@@ -198,6 +198,61 @@ def test_affine_strides_out_and_unlisted_rows():
         assert (engine.grouped_affine(x.t().contiguous().t(), groups, bank, lnorm=True) == y).all()
 
 
+@pytest.mark.parametrize("d_out", [1, 3, 77, 258])
+def test_affine_out_leaves_what_lies_behind_a_row(d_out):
+    torch = _torch()
+    from hyperion_amd import engine
+
+    r = _rng(17)
+    sizes = [3, 0, 150]
+    n, ld = sum(sizes), (d_out + 3) // 4 * 4 + 4
+    x = r.standard_normal((n, 9)).astype(np.float32)
+    groups = engine.RowGroups(sizes)
+    bank = engine.AffineBank(r.standard_normal((3, 9, d_out)), r.standard_normal((3, d_out)))
+    flat = torch.full(((n - 1) * ld + d_out,), 7.0, device="cuda")  # ends with the last row
+    out = flat.as_strided((n, d_out), (ld, 1))
+    for lnorm in (False, True):
+        want = engine.grouped_affine(torch.from_numpy(x).cuda(), groups, bank, lnorm=lnorm)
+        got = engine.grouped_affine(torch.from_numpy(x).cuda(), groups, bank, lnorm=lnorm, out=out)
+        assert got is out and torch.equal(got, want)
+    behind = torch.as_strided(flat[:-d_out], (n - 1, ld - d_out), (ld, 1), d_out)
+    assert torch.all(behind == 7.0)
+
+
+@pytest.mark.parametrize("d_out", [30, 300])
+@pytest.mark.parametrize("scale", [1e-24, 1e25])
+def test_affine_lnorm_of_rows_whose_squares_leave_fp32(scale, d_out):
+    """A product is off by less than 2^-20 of the sum of the magnitudes of its 20 terms, so a row's norm by 2^-20 of
+    their norm, which is some sqrt(20 * 2 / pi) < 4 times its own; the three roundings after that are below it."""
+    torch = _torch()
+    from hyperion_amd import engine
+
+    r = _rng(23)
+    x = r.standard_normal((5, 20))
+    W, sizes = r.standard_normal((2, 20, d_out)), [2, 3]
+    x32 = (x * scale).astype(np.float32)
+    y = np.concatenate([x32[:2].astype(np.float64) @ W[0].astype(np.float32), x32[2:].astype(np.float64) @ W[1].astype(np.float32)])
+    want = y * np.sqrt(d_out) / (np.linalg.norm(y, axis=1, keepdims=True) + 1e-10)
+    mags = np.concatenate([np.abs(x32[:2].astype(np.float64)) @ np.abs(W[0]), np.abs(x32[2:].astype(np.float64)) @ np.abs(W[1])])
+    bound = 2.0 ** -20 * mags * np.sqrt(d_out) / (np.linalg.norm(y, axis=1, keepdims=True) + 1e-10) + 2.0 ** -18 * np.abs(want)
+    got = engine.grouped_affine(torch.from_numpy(x32).cuda(), engine.RowGroups(sizes), engine.AffineBank(W), lnorm=True)
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= bound)
+
+
+def test_groups_keep_their_own_order():
+    torch = _torch()
+    from hyperion_amd import engine
+
+    r = _rng(29)
+    x = torch.from_numpy(r.standard_normal((6, 8)).astype(np.float32)).cuda()
+    order = torch.tensor([5, 0, 3, 1], dtype=torch.int32, device="cuda")
+    groups = engine.RowGroups([1, 3], order=order)
+    bank = engine.AffineBank(r.standard_normal((2, 8, 4)))
+    want = engine.grouped_affine(x, groups, bank)
+    order.fill_(2)
+    assert torch.equal(engine.grouped_affine(x, groups, bank), want)
+
+
 def test_affine_dims_of_each_group():
     torch = _torch()
     from hyperion_amd import engine
@@ -595,7 +650,6 @@ def test_refusals():
                 torch.zeros(6, 8, device="cuda")[:, 1:4], torch.zeros(6, 4, device="cuda").double()[:, :3]):
         refuses("out must be", engine.grouped_affine, x, g, bank, out=out)
     flat = torch.zeros(48, device="cuda")
-    refuses("no room", engine.grouped_affine, x, g, bank, out=torch.zeros(47, device="cuda").as_strided((6, 3), (8, 1), 4))
     refuses("share memory", engine.grouped_affine, flat.view(6, 8)[:, :4], g, bank, out=flat.view(6, 8)[:, 4:7])
     refuses(r"W must be", engine.AffineBank, np.ones((2, 4)))
     refuses(r"b must be", engine.AffineBank, np.ones((2, 4, 3)), np.ones((2, 4)))
@@ -610,6 +664,9 @@ def test_refusals():
     refuses("16-byte", engine.grouped_score, G[:, 1:33], G[:, 1:33], pairs)
     refuses("has 5 rows", engine.grouped_score, G[:5], G, pairs)
     refuses("out must be", engine.grouped_score, G, G, pairs, out=torch.zeros(21, device="cuda"))
+    refuses("share memory", engine.grouped_score, G, G, pairs, out=G.view(-1)[200:220])
+    refuses("rows", engine.RowGroups, [1 << 62, 1 << 62])
+    refuses("scores", engine.GroupPairs, *[engine.RowGroups([1 << 32])] * 2)
     refuses("expected one of", engine.grouped_gram64, x.half(), g)
     refuses("w must be", engine.grouped_gram64, x, g, torch.zeros(6, device="cuda"))
     refuses("no columns", engine.grouped_gram64, x[:, :0], g)
@@ -622,3 +679,4 @@ def test_refusals():
     refuses("not the groups", engine.q4_score, gallery, G, pairs)
     refuses("packed rows of 39", engine.q4_score, gallery, G[:, :39], one)
     refuses("out must be", engine.q4_score, gallery, G, one, out=torch.zeros(36, device="cuda", dtype=torch.float64))
+    refuses("share memory", engine.q4_score, gallery, G, one, out=G.view(-1)[:36])

@@ -118,6 +118,11 @@ def test_transform_bank_matches_the_chains():
     assert np.abs(z[ids == 0] - chains[0].predict(x[ids == 0])).max() <= 1e-4 * np.abs(z).max()
     only = TransformBank([LNorm(), LNorm()]).predict(x, ids % 2)
     assert np.abs(only - LNorm().predict(x)).max() <= 1e-5 * np.abs(only).max()
+    # chains that do nothing give a copy in fp32
+    same = TransformBank([[], []]).predict(dev.bfloat16(), ids % 2)
+    assert same.dtype == torch.float32 and torch.equal(same, dev.bfloat16().float())
+    same = TransformBank([[], []]).predict(dev, ids % 2)
+    assert torch.equal(same, dev) and same.data_ptr() != dev.data_ptr()
     for bad, match in ((lambda: bank.predict(x, ids[:-1]), "group ids for"), (lambda: bank.predict(x, ids + 1), "lie in"),
                        (lambda: TransformBank([]), "at least one"), (lambda: bank.predict(x[0], ids), "num_vectors, dim"),
                        (lambda: TransformBank([chains[0], LNorm()]).predict(x, ids % 2), "different"),

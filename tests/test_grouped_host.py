@@ -38,12 +38,13 @@ def test_sizes_of_tables():
 
 
 def test_refusals_of_the_c_abi():
-    def affine(x=P, kind=0, ldx=8, d=8, tile=64, w=P, m=4, y=P, ldy=4, n=1):
-        return _refused("hypmi_grouped_affine", x, kind, ldx, d, P, P, tile, n, 1, 1, None, w, P, None, m, 0, y, ldy, None)
+    def affine(x=P, kind=0, ldx=8, d=8, tile=64, w=P, m=4, y=P, ldy=4, n=1, cols=None):
+        return _refused("hypmi_grouped_affine", x, kind, ldx, d, P, P, tile, n, 1, 1, None, w, P, None, m, 0, y, ldy, m if cols is None else cols, None)
 
     assert "null" in affine(x=None) and "null" in affine(w=None) and "null" in affine(y=None)
     assert "fp32, fp16 or bf16" in affine(kind=3) and "fp32, fp16 or bf16" in affine(kind=-1)
     assert "leading" in affine(ldx=7) and "leading" in affine(ldy=6, m=6) and "leading" in affine(ldy=4, m=5)
+    assert "columns to write" in affine(cols=3) and "columns to write" in affine(m=2, cols=5, ldy=8)
     assert "16, 64 or 128" in affine(tile=48)
     assert "16-byte" in affine(y=ctypes.c_void_p(20))
     assert "bad shape" in affine(d=0) and "bad shape" in affine(n=-1)
@@ -81,10 +82,17 @@ def test_refusals_of_the_c_abi():
     assert "16, 32 or 64" in q4(tests=48) and "coordinates" in q4(k=0)
     assert "16-byte" in q4(codes=ctypes.c_void_p(8))
 
+    def pack(s=P, ld=8, k=8, n=1, c=P, out=P, kp=16):
+        return _refused("hypmi_grouped_pack", s, ld, k, P, 1, n, P, c, out, None, kp, None)
+
+    assert "null" in pack(s=None) and "null" in pack(c=None) and "no result" in pack(out=None)
+    assert "bad shape" in pack(ld=7) and "bad shape" in pack(kp=9) and "bad shape" in pack(k=0) and "bad shape" in pack(n=-1)
+
 
 def test_nothing_to_do_is_no_error():
     lib = _lib.load()
-    assert lib.hypmi_grouped_affine(None, 0, 8, 8, None, None, 64, 0, 0, 0, None, None, None, None, 4, 0, None, 4, None) == 0
+    assert lib.hypmi_grouped_affine(None, 0, 8, 8, None, None, 64, 0, 0, 0, None, None, None, None, 4, 0, None, 4, 4, None) == 0
+    assert lib.hypmi_grouped_pack(None, 8, 8, None, 0, 0, None, None, P, None, 16, None) == 0
     assert lib.hypmi_grouped_score(None, 40, None, 40, 40, None, None, None, None, 0, 0, None, None) == 0
     assert lib.hypmi_grouped_gram_f64(None, 0, 8, 8, None, None, None, None, 0, 0, 0, None, None, None, None, 0, None) == 0
     assert lib.hypmi_q4_score(None, None, None, 30, None, 32, None, None, None, None, None, 16, 64, 0, 0, None, None) == 0
