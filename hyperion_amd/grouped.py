@@ -16,6 +16,18 @@ _AFFINE_TILES = (16, 64, 128)
 _Q4_TESTS = (16, 32, 64)
 
 
+def _affine_tile(mean, d_in, d_out, itemsize):
+    """Rows per workgroup of the affine map, by the mean size of the groups.  Measured with 200 groups of ragged
+    sizes, tiles of 16 / 64 / 128 rows in us: fp32 200 -> 200 with 22 rows a group 15.5 / 16.7 / 18.6, with 37 rows
+    21.8 / 17.6 / 19.6, with 117 rows 46 / 23.5 / 26, with 195 rows 64 / 37 / 28.5.  fp32 rows that do not fit one
+    chunk of the tile of 64 (256 coordinates) keep two of 64 KB in shared memory, one workgroup per CU, which pays
+    only with few columns to multiply them with: 512 -> 200 with 64 rows 66 / 67 / 48, 512 -> 77 with 83 rows
+    29 / 23 / 27."""
+    if mean <= 20:
+        return 16
+    return 64 if mean <= 140 and (itemsize == 2 or d_in <= 256 or d_out <= 128) else 128
+
+
 def _prefix(counts):
     out = np.zeros(len(counts) + 1, dtype=np.int64)
     np.cumsum(counts, out=out[1:])
@@ -106,10 +118,7 @@ class RowGroups(_Plan):
         self._n_tiles = dict(zip(_AFFINE_TILES, (int(p[-1]) for p in prefix)))
         self._n_units, self._n_slots = int(units[-1]), int(slots[-1])
         self._order_ptr = None if self.order is None else self.order.data_ptr()
-        # rows per workgroup of the affine map: the largest tile that most rows can fill
-        used = int(np.count_nonzero(sizes))
-        mean = self.total / used if used else 0
-        self._affine_tile = 16 if mean <= 16 else 64 if mean <= 1000 else 128
+        self._mean = self.total / max(1, int(np.count_nonzero(sizes)))
         self._own(self._tab, self.order)
 
     @classmethod
@@ -177,10 +186,13 @@ class GroupPairs(_Plan):
         self.numel = int(self.offsets[-1])
         lib = _lib.load()
         span = lib.hypmi_grouped_score_span()
-        # tests per gallery task: the codes of a row are unpacked once per tile of tests, which costs about as much
-        # as multiplying them with 32 tests
-        cost = [float(np.sum(n2 * _ceil(n1, t) * (32.0 + t))) for t in _Q4_TESTS]
-        self._q4_tests = _Q4_TESTS[int(np.argmin(cost))]
+        # tests per gallery task: unpacking the codes of a row costs as much as multiplying them with 7 tests, and a
+        # tile is paid in full.  Tiles of 64 leave two waves per SIMD and pay where groups have hundreds of tests: a
+        # million rows x 1000 tests 1579 / 1345 / 1216 us with tiles of 16 / 32 / 64, x 64 tests 102.5 / 102.6 / 106;
+        # 200 000 rows x 48 tests 21.5 / 22.0 / 27.3, x 24 tests 17.7 / 17.0 / 24.8.
+        cost = [float(np.sum(n2 * _ceil(n1, t) * (7.0 + t))) for t in _Q4_TESTS[:2]]
+        many = self.numel >= 200 * max(1, int(n2.sum()))
+        self._q4_tests = 64 if many else _Q4_TESTS[int(np.argmin(cost))]
         # gallery rows per task: three workgroups on each of 256 CUs at once, or a whole number of such rounds
         work = int(np.sum(n2 * _ceil(n1, self._q4_tests)))
         rounds = max(1, _ceil(work, 768 * 4096))
@@ -316,7 +328,7 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
             raise ValueError("out must be fp32 [%d, %d] on %s with 16-byte aligned rows" % (n, d, x.device))
         if _overlap(x, y):
             raise ValueError("out must not share memory with x")
-    tile = groups._affine_tile
+    tile = _affine_tile(groups._mean, bank.d_in, d, x.element_size())
     n_tiles = groups._n_tiles[tile]
     if n_tiles:
         _run(_lib.load().hypmi_grouped_affine, x.device, (groups, bank), x.data_ptr(), kinds[x.dtype], ldx, bank.d_in,

@@ -90,12 +90,15 @@ AFFINE = [
     ([1500, 1029], 515, 64, True, False),
     ([7, 9], 1024, 512, True, False),
     ([0, 0], 8, 8, True, False),
-    # many rows a group: the kernel whose workgroups take several tiles
+    # many rows a group: tiles of 128
     ([40000, 0, 3000], 64, 20, True, False),
     ([2500, 1, 2700], 67, 256, True, True),
     ([1001, 1500], 190, 270, True, False),
     ([36000], 129, 33, False, True),
     ([3000, 1300, 2500], 321, 130, True, False),
+    # tiles of 64 over rows of several chunks
+    ([60, 21, 100], 700, 100, True, True),
+    ([30, 50, 1, 64], 300, 200, False, False),
 ]
 
 
@@ -495,6 +498,11 @@ Q4 = [
     ([5, 100], [1025, 70], 310),
     ([64, 2], [65, 64], 512),
     ([0, 0], [5, 6], 30),
+    # hundreds of tests: tiles of 64
+    ([300, 0, 9], [130, 5, 1], 150),
+    ([210], [70], 310),
+    ([257], [1100], 33),
+    ([250, 190], [65, 64], 512),
 ]
 
 
