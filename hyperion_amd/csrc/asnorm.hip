@@ -952,10 +952,10 @@ constexpr int GP_XCD_GROUPS = 16;  // row groups that share 128-byte lines of th
 // one rounding per operation in this order wherever it is computed (no contraction into fma), so that
 // the fused and the separate paths give the same bits.
 __device__ __forceinline__ float asnorm_value(float s, float mz, float iz, float mt, float it) {
-#pragma clang fp contract(off)  // __fmul_rn / __fadd_rn are plain operators here and would fuse into z + (s - mt) it
-    const float z = __fmul_rn(__fsub_rn(s, mz), iz);
-    const float t = __fmul_rn(__fsub_rn(s, mt), it);
-    return __fmul_rn(__fadd_rn(z, t), 0.70710678118654752440f);
+#pragma clang fp contract(off)  // for the operators of this block: __fmul_rn / __fadd_rn are plain operators of another
+    const float z = (s - mz) * iz;
+    const float t = (s - mt) * it;
+    return (z + t) * 0.70710678118654752440f;
 }
 
 // What the gather needs to finish the normalisation itself (rows = enrolment models, lists = tests):
