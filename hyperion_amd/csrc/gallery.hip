@@ -21,6 +21,10 @@
 // fp16 pairs (see score_split.hip), so a score is the fp32-accurate product of the row that the codes stand for.
 // The contraction of one instruction is one scale group: its result is multiplied by the scale and added up in
 // fp32.
+//
+// Measured at 150 coordinates: one test against a million rows 24 us (93 MB, 3.9 TB/s of a copy's 4.95), 1000 tests
+// 1.2 ms, 40 partitions of 500 to 30 000 rows with 0 to 40 tests each 13 us (two dependent reads and the
+// preparation of the tests come before the first product).
 #include "grouped.h"
 
 namespace hypmi_detail {

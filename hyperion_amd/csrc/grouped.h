@@ -53,7 +53,7 @@ __device__ __forceinline__ void split_pair4(f32x4 x, float up, f16x4& x0, f16x4&
 }
 
 // max(x, x of another lane) by a data-parallel-primitive control: 0xB1 lane ^ 1, 0x4E lane ^ 2, 0x141 the mirror
-// image within eight lanes, 0x140 within sixteen, 0x128 lane ^ 8
+// image within eight lanes, 0x140 within sixteen
 template <int CTRL>
 __device__ __forceinline__ float dpp_max(float x) {
     const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true);

@@ -16,6 +16,11 @@
 // taken from the chunk of coordinates at hand (largest magnitude to [2^8, 2^9)), kept while later chunks stay
 // below 2^15, and lowered otherwise, with the sums so far multiplied by the (exact) power of two.  Six
 // powers of two of headroom cost nothing: x1 keeps 2^-33 of the row's largest magnitude.
+//
+// Measured: 127 500 fp32 rows of 24 groups, 512 -> 150, 96 us (3.6 TB/s; the copy of as much 69); 115 700 bf16 rows of
+// 6 groups by an order, 512 -> 200, 99 us (2.2 TB/s; without the memory 68, without the products 88, without the
+// stores 94: the steps of a workgroup overlap only in part); 19 200 rows of 200 groups, 200 -> 77, normalised 13.4 us;
+// 12 rows of 8 groups, 512 -> 200, 9.7 us, the latency of table, row number, row and norm one after the other.
 #include "grouped.h"
 
 #include <type_traits>

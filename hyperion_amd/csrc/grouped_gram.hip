@@ -15,6 +15,12 @@
 // shared memory; in smaller ones every wave has a block of its own.  A group of more than GRAM_SPAN rows is cut into
 // chunks; every chunk writes its block to a slot of the workspace and a second kernel adds the slots in chunk order.
 // No sum depends on scheduling.
+//
+// Measured: 57 300 float64 rows of 7 groups, d = 512, 350 us and 9 for the second kernel (43 TFLOP/s; without the
+// loads 290); 25 600 fp32 rows of 200 groups, d = 200, 48 us, of which the matrix instructions are 20 and the writing
+// of 64 MB 13.  GRAM_SPLIT: with 200 groups of 96 rows a wave per block takes 32 us and four waves 44, with 384 and
+// more rows 47 to 60 and 50 to 48; the ragged groups above take 50.3 / 48.9 / 49.9 / 51.6 / 53.2 us with a limit of
+// 128 / 192 / 256 / 320 / 400 rows.  GRAM_SPAN: 2048 rows as fast and a second kernel of 13 us, 8192 rows 470 us.
 #include "grouped.h"
 
 #include <type_traits>

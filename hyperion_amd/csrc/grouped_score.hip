@@ -14,8 +14,8 @@
 // flight meanwhile.  Test rows are the first operand of the matrix instruction, so a lane ends up with four
 // neighbouring scores of one enrol row.
 //
-// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (25.8 M scores) 42 us, 12 domains of 300 to
-// 20000 test vectors (68.9 M scores) 120 to 135 us: 2.1 to 2.4 TB/s of results, 0.5 PFLOP/s of fp16 products.  What
+// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 42 us, 12 domains of 300 to
+// 20000 test vectors (68.9 M scores) 120 to 135 us: 2.0 to 2.3 TB/s of results, 0.5 PFLOP/s of fp16 products.  What
 // bounds it is the issue of instructions: of a tile's 3600 clocks per wave 960 are matrix instructions and 900 vector
 // ones, and two waves per SIMD hide little of either behind the other.  Without the matrix instructions the domains
 // take 53 us, without the stores 95, without the conversion 5 less; spans of 256 to 768, three waves per SIMD, tiles
