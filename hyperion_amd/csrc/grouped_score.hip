@@ -8,21 +8,21 @@
 // are converted here, on their way to the matrix instructions: a block has only as many columns as the group
 // has rows, so a converted copy of the operands would cost as much traffic as the scores themselves.
 //
-// A wave keeps 16 RT enrol rows as operands in registers and walks up to `span` test rows of its group in tiles of
-// 32 (a group's test rows are cut into equal parts), which the four waves of the workgroup load, convert (a row's
-// largest magnitude over eight lanes) and leave in LDS in operand order; the values of the next two tiles are in
-// flight meanwhile.  Test rows are the first operand of the matrix instruction, so a lane ends up with four
-// neighbouring scores of one enrol row.
+// A workgroup has four or eight waves that multiply and two that load.  A multiplying wave keeps 16 RT enrol rows as
+// operands in registers and walks up to `span` test rows of its group in tiles of 32 (a group's test rows are cut into
+// equal parts); the loading waves take 16 rows of the next tile each, a row by four lanes, find its largest magnitude,
+// convert it and leave it in LDS in operand order, and request the tile after that.  Memory operations of a wave
+// complete in order, so a wave that both stores scores and loads rows waits for its scores to be written: with four
+// waves that did both, 200 recordings took 42 us instead of 35 and 12 domains 117 instead of 107 at best.  Test rows
+// are the first operand of the matrix instruction, so a lane ends up with four neighbouring scores of one enrol row.
 //
-// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 42 us, 12 domains of 300 to
-// 20000 test vectors (68.9 M scores) 120 to 135 us: 2.0 to 2.3 TB/s of results, 0.5 PFLOP/s of fp16 products.  What
-// bounds it is the issue of instructions: of a tile's 3600 clocks per wave 960 are matrix instructions and 900 vector
-// ones, and two waves per SIMD hide little of either behind the other.  Without the matrix instructions the domains
-// take 53 us, without the stores 95, without the conversion 5 less; spans of 256 to 768, three waves per SIMD, tiles
-// fetched one or three ahead and stores of whole lines stay within 5 % of this.
+// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 35 us, 12 domains of 300 to
+// 20000 test vectors (68.9 M scores) 105 to 125 us: 2.2 to 2.6 TB/s of results.  The domains write 334 MB for 276 (a
+// row of a block starts anywhere in a line) and read 91 MB for 20, 3.4 TB/s together where a copy reaches 4.95;
+// without the stores they take 95 us, with the stores and one multiplication per span 76 to 85.  Enrol blocks in
+// turn instead of spans read 47 MB but leave the last workgroups alone for longer (114 us at best); spans of 256 to
+// 1024, 32 rows a wave (109 us), rows converted beforehand by a kernel of their own (131 + 10 us) are not faster.
 #include "grouped.h"
-
-#include <type_traits>
 
 namespace hypmi_detail {
 
@@ -44,12 +44,50 @@ struct ScoreArgs {
 constexpr int SCORE_RUN = 8;     // tasks dealt to an XCD at a time
 constexpr int SCORE_SPAN = 512;  // test rows one workgroup walks at most
 
-template <int KS, int RT>  // k-steps of 32 coordinates, row tiles of 16 per wave
-__global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
+// Coordinates 32 s + 8 kq .. + 7 of the row at `p`, s = 0 .. KS - 1; lanes r16 + 16 kq hold one row.  Past the end of a
+// row its last octet is read again, taken out by value in `operand`.
+template <int KS>
+struct RowValues {
+    f32x4 x[KS][2];
+
+    __device__ __forceinline__ void fetch(const float* p, int kp, int kq) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int k = 32 * s + 8 * kq, at = k < kp ? k : kp - 8;
+            x[s][0] = *reinterpret_cast<const f32x4*>(p + at);
+            x[s][1] = *reinterpret_cast<const f32x4*>(p + at + 4);
+        }
+    }
+
+    // exponent of the power of two that takes the row's largest magnitude to [2^14, 2^15)
+    __device__ __forceinline__ int scale() const {
+        float m = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(x[s][h][q]));
+        m = swap32_max(swap16_max(m));
+        const int up = m > 0.f ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
+        return up > 126 ? 126 : up;
+    }
+
+    __device__ __forceinline__ void operand(int s, float f, int kp, int kq, f16x8& a0, f16x8& a1) const {
+        const float fs = 32 * s + 8 * kq < kp ? f : 0.f;
+        f16x4 l0, l1, h0, h1;
+        split_pair4(x[s][0], fs, l0, l1);
+        split_pair4(x[s][1], fs, h0, h1);
+        a0 = __builtin_shufflevector(l0, h0, 0, 1, 2, 3, 4, 5, 6, 7);
+        a1 = __builtin_shufflevector(l1, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+template <int KS, int RT, int NW>  // k-steps of 32 coordinates, row tiles of 16 per wave, computing waves
+__global__ __launch_bounds__(64 * NW + 128, NW == 8 ? 5 : KS <= 8 ? 3 : 2) void grouped_score_kernel(ScoreArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int OCT = (4 * KS + 7) / 8;  // octets of coordinates per lane of the loading side
     __shared__ uint4 tile[2][2 * KS * 2 * 64];  // [buffer][(column tile, k-step, part, lane)]
-    __shared__ int scale[2][32];
+    __shared__ __attribute__((aligned(16))) int scale[2][32];
 
     const int64_t t = xcd_task(blockIdx.x, g.n_tasks, SCORE_RUN);
     if (t < 0) return;
@@ -61,136 +99,95 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
     const int64_t span = ((n2 + spans - 1) / spans + 31) & ~31LL;  // equal parts, at most g.span
     const int64_t j_beg = (task - i_blk * spans) * span;
     const int ncol = n2 - j_beg < span ? (int)(n2 - j_beg) : (int)span;
+    const int tiles = (ncol + 31) >> 5;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, kq = lane >> 4;
-    const float* G2 = g.G2 + (g.off2[e] + j_beg) * g.ld2;
 
-    // ---- test side: lane loads octets (lane >> 3) + 8 o of row 8 wave + (lane & 7) of a tile
-    const int lr = 8 * wave + (lane & 7), lo = lane >> 3;
-    typedef f32x4 Octets[OCT][2];
-    Octets v, u;
-    // Every call issues the same loads, so that the waits for one tile's values are counted past those of the next
-    // and past stores: behind the last row the last row is read again, behind the last octet the last octet (taken
-    // out by value in `store`).
-    int oct_at[OCT];
+    if (wave >= NW) {
+        // ---- a loading wave: rows 16 c .. + 15 of every tile
+        const int c = wave - NW;
+        const float* G2 = g.G2 + (g.off2[e] + j_beg) * g.ld2;
+        RowValues<KS> v;
+        auto fetch = [&](int it) {
+            const int j = 32 * it + 16 * c + r16;
+            v.fetch(G2 + (int64_t)(j < ncol ? j : ncol - 1) * g.ld2, g.kp, kq);
+        };
+        auto store = [&](int buf) {
+            const int up = v.scale();
+            if (kq == 0) scale[buf][16 * c + r16] = up;
+            const float f = exp2_int(up);
 #pragma unroll
-    for (int o = 0; o < OCT; ++o) oct_at[o] = 8 * (lo + 8 * o) < g.kp ? 8 * (lo + 8 * o) : g.kp - 8;
-    auto fetch = [&](Octets& v, int tile) {
-        const int j = 32 * tile + lr < ncol ? 32 * tile + lr : ncol - 1;
-        const float* p = G2 + j * g.ld2;
-#pragma unroll
-        for (int o = 0; o < OCT; ++o) {
-            v[o][0] = *reinterpret_cast<const f32x4*>(p + oct_at[o]);
-            v[o][1] = *reinterpret_cast<const f32x4*>(p + oct_at[o] + 4);
+            for (int s = 0; s < KS; ++s) {
+                f16x8 a0, a1;
+                v.operand(s, f, g.kp, kq, a0, a1);
+                uint4* dst = &tile[buf][((c * KS + s) * 2) * 64 + lane];
+                dst[0] = __builtin_bit_cast(uint4, a0);
+                dst[64] = __builtin_bit_cast(uint4, a1);
+            }
+        };
+        fetch(0);
+        store(0);
+        fetch(1);
+        __syncthreads();
+        for (int it = 0; it < tiles; ++it) {
+            if (it + 1 < tiles) {
+                store((it + 1) & 1);
+                fetch(it + 2);
+            }
+            __syncthreads();
         }
-    };
-    auto store = [&](const Octets& v, int buf) {
-        float m = 0.f;
-#pragma unroll
-        for (int o = 0; o < OCT; ++o)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(v[o][h][q]));
-#pragma unroll
-        for (int x = 8; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-        int up = m > 0.f ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
-        up = up > 126 ? 126 : up;
-        if (lo == 0) scale[buf][lr] = up;
-        const float f = exp2_int(up);
-        const int ct = lr >> 4, row = lr & 15;
-#pragma unroll
-        for (int o = 0; o < OCT; ++o) {
-            const int oct = lo + 8 * o;
-            if (oct >= 4 * KS) continue;
-            const float fo = 8 * oct < g.kp ? f : 0.f;
-            const int s = oct >> 2, q = oct & 3;
-            f16x4 a0, a1, b0, b1;
-            split_pair4(v[o][0], fo, a0, a1);
-            split_pair4(v[o][1], fo, b0, b1);
-            f16x4* dst = reinterpret_cast<f16x4*>(&tile[buf][((ct * KS + s) * 2) * 64 + q * 16 + (row ^ (8 * (q & 1)))]);
-            dst[0] = a0;
-            dst[1] = b0;
-            dst[128] = a1;
-            dst[129] = b1;
-        }
-    };
-
-    fetch(v, 0);
-    fetch(u, 1);
-    __builtin_amdgcn_sched_barrier(0);
+        return;
+    }
 
     // ---- enrol side: a[i][s][part] = coordinates 32 s + 8 kq .. + 7 of row i0 + 16 i + r16
-    const int64_t i0 = (i_blk * 4 + wave) * (16 * RT);
+    const int64_t i0 = (i_blk * NW + wave) * (16 * RT);
+    const bool live = i0 < n1;  // this wave has rows
     f16x8 a[RT][KS][2];
     int rs[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        int64_t row = i0 + 16 * i + r16;
-        row = row < n1 ? row : n1 - 1;
-        const float* p = g.G1 + (g.off1[e] + row) * g.ld1 + 8 * kq;
-        f32x4 x[KS][2];
-        float m = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (32 * s + 8 * kq < g.kp) {
-                x[s][0] = *reinterpret_cast<const f32x4*>(p + 32 * s);
-                x[s][1] = *reinterpret_cast<const f32x4*>(p + 32 * s + 4);
-            } else {
-                x[s][0] = x[s][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(x[s][h][q]));
-        }
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        int up = m > 0.f ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
-        up = up > 126 ? 126 : up;
-        rs[i] = up;
-        const float f = exp2_int(up);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            f16x4 a0, a1, b0, b1;
-            split_pair4(x[s][0], f, a0, a1);
-            split_pair4(x[s][1], f, b0, b1);
-            a[i][s][0] = __builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7);
-            a[i][s][1] = __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-    }
-    const int xs = kq * 16 + (r16 ^ (8 * (kq & 1)));
     // result rows of this lane; a row past the end holds the last row's scores (its operand is a copy) and stores
     // them to the same place, so that no store depends on a comparison
     float* dst[RT];
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int64_t row = i0 + 16 * i + r16;
-        dst[i] = g.S + g.blocks[e] + (row < n1 ? row : n1 - 1) * n2 + j_beg + 4 * kq;
+        for (int i = 0; i < RT; ++i) {
+            int64_t row = i0 + 16 * i + r16;
+            row = row < n1 ? row : n1 - 1;
+            dst[i] = g.S + g.blocks[e] + row * n2 + j_beg + 4 * kq;
+            RowValues<KS> v;
+            v.fetch(g.G1 + (g.off1[e] + row) * g.ld1, g.kp, kq);
+            rs[i] = v.scale();
+            const float f = exp2_int(rs[i]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) v.operand(s, f, g.kp, kq, a[i][s][0], a[i][s][1]);
+        }
     }
     auto multiply = [&](int it, bool whole) {
         const int buf = it & 1;
         f32x4 acc[RT][2];
 #pragma unroll
         for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        f16x8 b[2][2][2];  // [k-step parity][column tile][part]
+        auto request = [&](int s) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint4* p = &tile[buf][((c * KS + s) * 2) * 64 + xs];
-                const f16x8 b0 = __builtin_bit_cast(f16x8, p[0]);
-                const f16x8 b1 = __builtin_bit_cast(f16x8, p[64]);
+                for (int p = 0; p < 2; ++p)
+                    b[s & 1][c][p] = __builtin_bit_cast(f16x8, tile[buf][((c * KS + s) * 2 + p) * 64 + lane]);
+        };
+        request(0);
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
-                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1, a[i][s][0], acc[i][c], 0, 0, 0);
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) request(s + 1);
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
-                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][1], acc[i][c], 0, 0, 0);
+            for (int p = 0; p < 3; ++p)
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
-                    acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0, a[i][s][0], acc[i][c], 0, 0, 0);
-            }
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < RT; ++i)
+                        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[s & 1][c][p == 0], a[i][s][p == 1],
+                                                                           acc[i][c], 0, 0, 0);
+        }
         // lane: columns 32 it + 16 c + 4 kq .. + 3 of enrol row i0 + 16 i + r16
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -211,40 +208,25 @@ __global__ __launch_bounds__(256) void grouped_score_kernel(ScoreArgs g) {
             }
         }
     };
-
-    auto walk = [&](auto live_tag) {
-        constexpr bool LIVE = decltype(live_tag)::value;  // this wave has rows
-        store(v, 0);
-        fetch(v, 2);
-        __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    const int whole = ncol >> 5;
+    for (int it = 0; it < whole; ++it) {
+        if (live) multiply(it, true);
         __syncthreads();
-        const int whole = ncol >> 5;
-        for (int it = 0; it < whole; it += 2) {
-            if (LIVE) multiply(it, true);
-            store(u, 1);
-            fetch(u, it + 3);
-            __builtin_amdgcn_sched_barrier(0);
-            __syncthreads();
-            if (it + 1 == whole) break;
-            if (LIVE) multiply(it + 1, true);
-            store(v, 0);
-            fetch(v, it + 4);
-            __builtin_amdgcn_sched_barrier(0);
-            __syncthreads();
-        }
-        if (LIVE && 32 * whole < ncol) multiply(whole, false);
-    };
-    if (i0 < n1) walk(std::true_type{});
-    else walk(std::false_type{});
+    }
+    if (whole < tiles) {
+        if (live) multiply(whole, false);
+        __syncthreads();
+    }
 #endif
 }
 
 template <int KS>
 int launch_score(const ScoreArgs& g, hipStream_t stream) {
-    constexpr int RT = KS <= 6 ? 2 : 1;
+    constexpr int RT = KS == 6 ? 2 : 1, NW = KS <= 5 ? 8 : 4;
     const int64_t grid = xcd_grid(g.n_tasks, SCORE_RUN);
     HYPMI_REQUIRE(grid <= 0x7fffffffLL, "grouped_score: too many workgroups");
-    hipLaunchKernelGGL((grouped_score_kernel<KS, RT>), dim3((unsigned)grid), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((grouped_score_kernel<KS, RT, NW>), dim3((unsigned)grid), dim3(64 * NW + 128), 0, stream, g);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
 }

@@ -310,6 +310,11 @@ SCORE = [
     ([66], [35], 376),
     ([20, 90], [90, 33], 512),
     ([1, 1], [2000, 1], 40),
+    ([200, 17], [40, 600], 72),
+    ([70], [90], 128),
+    ([130, 5], [70, 33], 176),
+    ([33], [40], 264),
+    ([18, 65], [33, 1], 392),
 ]
 
 
