@@ -242,6 +242,23 @@ def test_affine_lnorm_of_rows_whose_squares_leave_fp32(scale, d_out):
     assert np.all(np.abs(got.double().cpu().numpy() - want) <= bound)
 
 
+def test_no_groups():
+    torch = _torch()
+    from hyperion_amd import engine
+
+    none = engine.RowGroups([])
+    x = torch.zeros(0, 12, device="cuda")
+    assert engine.grouped_affine(x, none, engine.AffineBank(np.zeros((0, 12, 5))), lnorm=True).shape == (0, 5)
+    C, F = engine.grouped_gram64(x, none)
+    assert C.shape == (0, 12, 12) and F.shape == (0, 12)
+    G = torch.zeros(0, 40, device="cuda")
+    pairs = engine.GroupPairs(none, none)
+    assert engine.grouped_score(G, G, pairs).numel() == 0 and pairs.blocks(engine.grouped_score(G, G, pairs)) == []
+    assert engine.q4_score(engine.q4_rows(G, 30, none), G, pairs).numel() == 0
+    assert engine.grouped_pack(x, none, np.zeros((0, 4, 12)), np.zeros(0))[0].shape[0] == 0
+    assert engine.RowGroups.from_ids([], 3).sizes.tolist() == [0, 0, 0]
+
+
 def test_groups_keep_their_own_order():
     torch = _torch()
     from hyperion_amd import engine
