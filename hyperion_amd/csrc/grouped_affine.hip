@@ -18,9 +18,9 @@
 // powers of two of headroom cost nothing: x1 keeps 2^-33 of the row's largest magnitude.
 //
 // Measured: 127 500 fp32 rows of 24 groups, 512 -> 150, 96 us (3.6 TB/s; the copy of as much 69); 115 700 bf16 rows of
-// 6 groups by an order, 512 -> 200, 99 us (2.2 TB/s; without the memory 68, without the products 88, without the
+// 6 groups by an order, 512 -> 200, 97 us (2.2 TB/s; without the memory 68, without the products 88, without the
 // stores 94: the steps of a workgroup overlap only in part); 19 200 rows of 200 groups, 200 -> 77, normalised 13.4 us;
-// 12 rows of 8 groups, 512 -> 200, 9.7 us, the latency of table, row number, row and norm one after the other.
+// 12 rows of 8 groups, 512 -> 200, 9.0 us, the latency of table, row number, row and norm one after the other.
 #include "grouped.h"
 
 #include <type_traits>
@@ -192,7 +192,8 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     // the chunk loop of a wave with `tiles` column tiles
     auto walk = [&](auto tiles_tag) {
         constexpr int N = decltype(tiles_tag)::value;
-        constexpr int WS = RT == 8 ? 1 : RT == 4 ? 2 : 4;  // k-steps of weights in registers
+        // k-steps of weights in registers; 4 and 8 with tiles of 16 take 9.7 and 10.3 us for the twelve rows above, 2 takes 9.0
+        constexpr int WS = RT == 8 ? 1 : 2;
         const uint4* w0p = wp + ((int64_t)e * g.ct + ct0) * w_tile;
         const uint4* w1p = wp + ((int64_t)e * g.ct + ct1) * w_tile;
         f16x8 w[WS][N > 0 ? N : 1][2];
@@ -224,9 +225,11 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x0, acc[i][j], 0, 0, 0);
             }
         };
+        fetch(0);  // first: converting the rows waits for nothing else
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < WS; ++s) weights(s, s);
-        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
         store(0, 0);
         __syncthreads();
         for (int ch = 0; ch < chunks; ++ch) {

@@ -340,14 +340,11 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
 
 def _overlap(a, b):
     """Whether the storage ranges of two tensors meet."""
-    def span(t):
-        if t.numel() == 0:
-            return 0, 0
-        lo = t.data_ptr()
-        return lo, lo + t.element_size() * (1 + sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())))
+    def end(t):
+        last = sum([(s - 1) * st for s, st in zip(t.shape, t.stride())])
+        return t.data_ptr() + t.element_size() * (1 + last)
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def _packed(G, groups, what):
@@ -388,8 +385,9 @@ def grouped_pack(s, groups, maps, c, sides="both"):
 def grouped_score(G1, G2, pairs, out=None):
     """Scores of packed enrol rows against packed test rows of the same group (Plan.prologue, both [n, kp]):
     the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e)."""
+    same = G2 is G1 and pairs.cols is pairs.rows  # self-scores: checked once
     G1, ld1 = _packed(G1, pairs.rows, "G1")
-    G2, ld2 = _packed(G2, pairs.cols, "G2")
+    G2, ld2 = (G1, ld1) if same else _packed(G2, pairs.cols, "G2")
     kp = G1.shape[1]
     if G2.shape[1] != kp:
         raise ValueError("packed widths differ: %d vs %d" % (kp, G2.shape[1]))
