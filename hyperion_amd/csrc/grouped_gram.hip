@@ -13,14 +13,15 @@
 // Groups differ in size by orders of magnitude, and a wave with a thousand rows runs for 25 us: a chunk of more than
 // GRAM_SPLIT rows is therefore shared by the four waves of a workgroup, a quarter each, which add their blocks in
 // shared memory; in smaller ones every wave has a block of its own.  A group of more than GRAM_SPAN rows is cut into
-// chunks; every chunk writes its block to a slot of the workspace and a second kernel adds the slots in chunk order.
-// No sum depends on scheduling.
+// chunks of one length; every chunk writes its block to a slot of the workspace and a second kernel adds the slots in
+// chunk order.  No sum depends on scheduling.
 //
-// Measured: 57 300 float64 rows of 7 groups, d = 512, 350 us and 9 for the second kernel (43 TFLOP/s; without the
-// loads 290); 25 600 fp32 rows of 200 groups, d = 200, 48 us, of which the matrix instructions are 20 and the writing
-// of 64 MB 13.  GRAM_SPLIT: with 200 groups of 96 rows a wave per block takes 32 us and four waves 44, with 384 and
-// more rows 47 to 60 and 50 to 48; the ragged groups above take 50.3 / 48.9 / 49.9 / 51.6 / 53.2 us with a limit of
-// 128 / 192 / 256 / 320 / 400 rows.  GRAM_SPAN: 2048 rows as fast and a second kernel of 13 us, 8192 rows 470 us.
+// Measured: 57 300 float64 rows of 7 groups, d = 512, 299 us back to back, 14 of them the second kernel (50 TFLOP/s);
+// 25 600 fp32 rows of 200 groups, d = 200, 48 us, of which the matrix instructions are 20 and the writing of 64 MB 13.
+// GRAM_SPLIT: with 200 groups of 96 rows a wave per block takes 32 us and four waves 44, with 384 and more rows 47 to
+// 60 and 50 to 48; the ragged groups above take 50.3 / 48.9 / 49.9 / 51.6 / 53.2 us with a limit of 128 / 192 / 256 /
+// 320 / 400 rows.  GRAM_SPAN of 1024 / 1536 / 2048 / 3072 / 4096 rows: 316 / 312 / 299 / 302 / 324 us of the first
+// case (345 with 4096 and chunks that are full but for the last).
 #include "grouped.h"
 
 #include <type_traits>
@@ -45,7 +46,7 @@ struct GramArgs {
     int nb, pairs;
 };
 
-constexpr int GRAM_SPAN = 4096;  // rows of one chunk
+constexpr int GRAM_SPAN = 2048;  // rows of one chunk at most
 constexpr int GRAM_SPLIT = 192;  // a chunk of more rows is shared by four waves
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -81,10 +82,11 @@ __global__ __launch_bounds__(256, 2) void grouped_gram_kernel(GramArgs g) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int e = find_group(g.units, g.n_groups, unit);
     const int64_t u0 = unit - g.units[e], s_lim = g.offsets[e + 1], size = s_lim - g.offsets[e];
-    // whole chunks have four units each, so that the remainder starts at a multiple of four
-    const int64_t ch = u0 >> 2;
-    int64_t s_beg = g.offsets[e] + ch * GRAM_SPAN;
-    int ns = s_lim - s_beg < GRAM_SPAN ? (int)(s_lim - s_beg) : GRAM_SPAN;
+    // all chunks but the last have four units each; the chunks of a group are of one length
+    const int64_t ch = u0 >> 2, cut = size > GRAM_SPAN ? (size + GRAM_SPAN - 1) / GRAM_SPAN : 1;
+    const int64_t span = ((size + cut - 1) / cut + 63) & ~63LL;  // at most GRAM_SPAN where cut > 1
+    int64_t s_beg = g.offsets[e] + ch * span;
+    int ns = s_lim - s_beg < span ? (int)(s_lim - s_beg) : (int)span;
     const bool split = ns > GRAM_SPLIT;
     const int pair = quad * 4 + (split ? (int)(u0 & 3) : wave);
     if (pair >= g.pairs) return;  // the whole workgroup where the chunk is shared

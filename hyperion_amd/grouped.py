@@ -108,9 +108,11 @@ class RowGroups(_Plan):
             self._set_order(order)
         lib = _lib.load()
         span, split = lib.hypmi_grouped_gram_span(), lib.hypmi_grouped_gram_split()
-        cut, rest = _ceil(sizes, span), sizes % span
+        cut = _ceil(sizes, span)
+        # chunks of one length; the last may be short
+        rest = sizes - (np.maximum(cut, 1) - 1) * round_up(_ceil(sizes, np.maximum(cut, 1)), 64)
         prefix = [_prefix(_ceil(sizes, t)) for t in _AFFINE_TILES]
-        units = _prefix(4 * (sizes // span) + np.where(rest > split, 4, (rest > 0) | (sizes == 0)))
+        units = _prefix(4 * (np.maximum(cut, 1) - 1) + np.where(rest > split, 4, 1))
         slots = _prefix(np.where(cut > 1, cut, 0))
         self._tab = _tables([self.offsets] + prefix + [units, slots], self.device)
         base = self._tab.data_ptr()

@@ -578,9 +578,10 @@ int hypmi_grouped_score(const float* G1, int64_t ld1, const float* G2, int64_t l
 
 /* C_e = sum_r w_r x_r x_r^T [d x d] and F_e = sum_r w_r x_r [d] over the rows of every group, in float64 (w NULL:
  * 1; indexed by row of x).  x: HYPMI_F32 or HYPMI_F64.  C [n_groups x d x d] is exactly symmetric, empty groups
- * are zero, and the sums are added in a fixed order (same bits from run to run).  A group is cut into chunks of
- * hypmi_grouped_gram_span() rows; a chunk of more than hypmi_grouped_gram_split() rows counts four units, a smaller
- * one (and that of an empty group) one.  units: prefix sums of the groups' units; slots: prefix sums of the number of
+ * are zero, and the sums are added in a fixed order (same bits from run to run).  A group of s rows is cut into
+ * n = ceil(s / hypmi_grouped_gram_span()) chunks of ceil(s / n) rows, rounded up to 64 (the last is what is left); a
+ * chunk of more than hypmi_grouped_gram_split() rows counts four units, a smaller one (and that of an empty group)
+ * one: all but a group's last count four.  units: prefix sums of the groups' units; slots: prefix sums of the number of
  * chunks of the groups that have several, 0 for the others.  workspace: hypmi_grouped_gram_workspace_bytes(n_slots, d)
  * bytes, 8-byte aligned. */
 int hypmi_grouped_gram_span(void);

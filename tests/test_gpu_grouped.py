@@ -405,6 +405,8 @@ GRAM = [
     ([0, 0], 9),
     ([192, 193, 256, 4095], 50),
     ([4096, 4097, 4289, 0, 8192], 20),
+    ([2048, 2049, 2112, 0, 6145], 20),
+    ([59521, 1], 6),  # thirty chunks, the last of 129 rows
 ]
 
 
