@@ -20,7 +20,7 @@
 // 25 600 fp32 rows of 200 groups, d = 200, 48 us, of which the matrix instructions are 20 and the writing of 64 MB 13.
 // GRAM_SPLIT: with 200 groups of 96 rows a wave per block takes 32 us and four waves 44, with 384 and more rows 47 to
 // 60 and 50 to 48; the ragged groups above take 50.3 / 48.9 / 49.9 / 51.6 / 53.2 us with a limit of 128 / 192 / 256 /
-// 320 / 400 rows.  GRAM_SPAN of 1024 / 1536 / 2048 / 3072 / 4096 rows: 316 / 312 / 299 / 302 / 324 us of the first
+// 320 / 400 rows.  GRAM_SPAN of 1024 / 1536 / 2048 / 4096 rows: 316 / 312 / 299 / 324 us of the first
 // case (345 with 4096 and chunks that are full but for the last).
 #include "grouped.h"
 
