@@ -25,7 +25,8 @@ class AffineTransform(HypModel):
         return A, b, self._lnorm
 
     def _params_key(self):
-        return fingerprint(self.mu, self.T)
+        """What a device plan made from this transform is kept by: the type says what is done with mu and T."""
+        return (type(self), self._lnorm) + fingerprint(self.mu, self.T)
 
     def predict(self, x):
         return run_chain([self], x)

@@ -47,6 +47,10 @@ class TransformBank(HypModel):
             d = out
         return layers
 
+    def _key(self, d_in, device):
+        """What the maps laid out on the device are kept by: every chain's transforms, chain by chain."""
+        return d_in, device, tuple(tuple(t._params_key() for t in c) for c in self.chains)
+
     def predict(self, x, ids):
         """x [n, d] (host array, or a device tensor of fp32, fp16 or bf16), ids [n] host integers or a
         RowGroups over the rows of x: [n, d_out], a host array for a host array and a device fp32 tensor for a
@@ -61,7 +65,7 @@ class TransformBank(HypModel):
             y = engine.upload(x)
         else:
             y = x
-        key = (y.shape[1], y.device, tuple(t._params_key() for c in self.chains for t in c))
+        key = self._key(y.shape[1], y.device)
         if self._banks is None or self._banks_key != key:
             self._banks = [(engine.AffineBank(W, b, dims=dims, device=y.device), lnorm)
                            for W, b, dims, lnorm in self._layers(y.shape[1])]
