@@ -5,8 +5,9 @@ block of scores, in one launch.  The names here are part of hyperion_amd.engine.
 A batch is described once, by a RowGroups (sizes on the host, tables on the device) and, for products of
 two sides, a GroupPairs; the operators themselves neither wait for the device nor send it anything, so they
 can be captured in a HIP graph.  Inputs have to be on one device; the work runs on that device's current
-stream.  A RowGroups or GroupPairs can be used on any stream at once; an AffineBank and a Q4Rows are filled by
-launches on the stream they are made on, for which another stream waits as for any tensor."""
+stream.  A RowGroups, a GroupPairs and an AffineBank are complete when they have been made (which waits for the
+current stream) and can be used on any stream at once; a Q4Rows is filled by a launch on the stream it is made on, for
+which another stream waits as for any tensor."""
 import numpy as np
 
 from . import _lib
@@ -230,7 +231,8 @@ class AffineBank(_Plan):
     """One affine map per group, x -> x W[e] + b[e], laid out for grouped_affine.  W [E, d_in, d_out] and b
     [E, d_out] (or None), host arrays or device tensors of any float type, kept at fp32 accuracy.  dims
     [E] (optional): dimension of every map where they differ; W[e][:, dims[e]:] and b[e][dims[e]:] have to be
-    zero, and the length normalisation scales to sqrt(dims[e])."""
+    zero, and the length normalisation scales to sqrt(dims[e]).  The maps are laid out by the time the constructor
+    returns, so that any stream can use them at once; made while a HIP graph is captured they are part of the graph."""
 
     def __init__(self, W, b=None, dims=None, device=None):
         torch = _torch()
@@ -262,6 +264,9 @@ class AffineBank(_Plan):
         if self.num_groups:
             _run(lib.hypmi_grouped_weights, self.device, (), _ptr(W), None if b is None else _ptr(b), *args,
                  _ptr(self._w), _ptr(self._c))
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
 
     def _fp32(self, a):
         torch = _torch()

@@ -16,15 +16,14 @@ class TransformBank(HypModel):
     The chains have to take the same input dimension, to give the same output dimension and to normalise lengths
     the same number of times; dimensions in between may differ."""
 
-    _cache_defaults = {"_banks": lambda: None, "_banks_key": lambda: None}
+    _cache_defaults = {"_banks": lambda: (None, None)}
 
     def __init__(self, chains, **kwargs):
         super().__init__(**kwargs)
         if not chains:
             raise ValueError("a TransformBank needs at least one chain")
         self.chains = [list(getattr(c, "transforms", c if isinstance(c, (list, tuple)) else [c])) for c in chains]
-        self._banks = None
-        self._banks_key = None
+        self._banks = (None, None)  # key, maps: replaced together, so that a concurrent call sees both or neither
 
     def _layers(self, d_in):
         """[(W [E, d_in, d_out], b [E, d_out], dims or None, lnorm)] of the folded chains, float64."""
@@ -66,17 +65,18 @@ class TransformBank(HypModel):
         else:
             y = x
         key = self._key(y.shape[1], y.device)
-        if self._banks is None or self._banks_key != key:
-            self._banks = [(engine.AffineBank(W, b, dims=dims, device=y.device), lnorm)
-                           for W, b, dims, lnorm in self._layers(y.shape[1])]
-            self._banks_key = key
+        kept, banks = self._banks
+        if kept != key:
+            banks = [(engine.AffineBank(W, b, dims=dims, device=y.device), lnorm)
+                     for W, b, dims, lnorm in self._layers(y.shape[1])]
+            self._banks = key, banks
         if not isinstance(ids, engine.RowGroups):
             if len(ids) != y.shape[0]:
                 raise ValueError("%d group ids for %d rows" % (len(ids), y.shape[0]))
             ids = engine.RowGroups.from_ids(ids, len(self.chains), device=y.device)
-        for bank, lnorm in self._banks:
+        for bank, lnorm in banks:
             y = engine.grouped_affine(y, ids, bank, lnorm=lnorm)
-        if not self._banks:  # chains that do nothing
+        if not banks:  # chains that do nothing
             ids._check(y, "x")
             y = y.to(torch.float32, copy=True)
         return y if is_dev else engine.to_host(y, float_cpu())
