@@ -22,12 +22,21 @@ class PLDAGallery:
     def __init__(self, plda, preproc=None):
         self.plda = plda
         self.plan = plda.score_plan(preproc)
-        self.rows = None       # device int64: row of the enrolled array that a gallery row was made from
-        self.gallery = None
+        # (4-bit rows, device int64: row of the enrolled array that each was made from), replaced together
+        self._enrolled = None, None
+
+    @property
+    def gallery(self):
+        return self._enrolled[0]
+
+    @property
+    def rows(self):
+        return self._enrolled[1]
 
     def enrol(self, x, partition=None, num_partitions=None):
         """Replaces the gallery by the vectors x [n, d] (host array or device tensor); partition: number of every
-        vector's partition, 0 .. num_partitions - 1.  Returns self."""
+        vector's partition, 0 .. num_partitions - 1.  Waits until the gallery is written, so that any stream can search it at
+        once.  Returns self."""
         torch = engine.require_gpu()
         x = engine.upload(x)
         if partition is None:
@@ -38,15 +47,20 @@ class PLDAGallery:
             g = engine.RowGroups.from_ids(partition, num_partitions, device=x.device)
             groups, order = engine.RowGroups(g.sizes, device=x.device), g.order.long()
         G = self.plan.prologue(x, SIDE_ENROL)
-        self.rows = torch.arange(x.shape[0], device=x.device) if order is None else order
-        self.gallery = engine.q4_rows(G if order is None else G[order], self.plan.k, groups)
+        rows = torch.arange(x.shape[0], device=x.device) if order is None else order
+        gallery = engine.q4_rows(G if order is None else G[order], self.plan.k, groups)
+        torch.cuda.current_stream(x.device).synchronize()
+        self._enrolled = gallery, rows
         return self
 
     def _score(self, x, partition):
-        if self.gallery is None:
+        gallery, rows = self._enrolled
+        if gallery is None:
             raise ValueError("nothing is enrolled")
         x = engine.upload(x)
-        groups, order = self.gallery.groups, None
+        # a concurrent enrol may drop the rows while this stream reads them
+        rows.record_stream(engine.require_gpu().cuda.current_stream(rows.device))
+        groups, order = gallery.groups, None
         if partition is None:
             if groups.num_groups != 1:
                 raise ValueError("the gallery has %d partitions: say which one every test vector belongs to"
@@ -59,7 +73,7 @@ class PLDAGallery:
             tests, order = engine.RowGroups(g.sizes, device=x.device), g.order.long()
         G = self.plan.prologue(x, SIDE_TEST)
         pairs = engine.GroupPairs(tests, groups)
-        return pairs, order, engine.q4_score(self.gallery, G if order is None else G[order], pairs)
+        return pairs, order, rows, engine.q4_score(gallery, G if order is None else G[order], pairs)
 
     def llr(self, x, partition=None):
         """Scores of the test vectors x [m, d].  Without partitions [n, m], enrolled vectors by test vectors, as
@@ -67,7 +81,7 @@ class PLDAGallery:
         list of (rows of the enrolled array, rows of x, [rows, tests] scores), one per partition."""
         torch = engine.require_gpu()
         is_dev = isinstance(x, torch.Tensor)
-        pairs, order, flat = self._score(x, partition)
+        pairs, order, enrolled, flat = self._score(x, partition)
 
         def host(t):
             return t if is_dev else t.cpu().numpy() if t.dtype == torch.int64 else engine.to_host(t, float_cpu())
@@ -77,7 +91,7 @@ class PLDAGallery:
         res = []
         for e in range(pairs.rows.num_groups):
             g, t = pairs.cols.offsets, pairs.rows.offsets
-            res.append((host(self.rows[g[e]:g[e + 1]]), host(order[t[e]:t[e + 1]]), host(pairs.block(flat, e).t())))
+            res.append((host(enrolled[g[e]:g[e + 1]]), host(order[t[e]:t[e + 1]]), host(pairs.block(flat, e).t())))
         return res
 
     def identify(self, x, nbest=10, partition=None):
@@ -88,7 +102,7 @@ class PLDAGallery:
         is_dev = isinstance(x, torch.Tensor)
         if nbest < 1:
             raise ValueError("nbest must be at least 1")
-        pairs, order, flat = self._score(x, partition)
+        pairs, order, enrolled, flat = self._score(x, partition)
         m = pairs.rows.total
         rows = torch.full((m, nbest), -1, dtype=torch.int64, device=flat.device)
         best = torch.full((m, nbest), -np.inf, dtype=torch.float32, device=flat.device)
@@ -102,5 +116,5 @@ class PLDAGallery:
             t0, t1 = int(pairs.rows.offsets[e]), int(pairs.rows.offsets[e + 1])
             at = slice(t0, t1) if order is None else order[t0:t1]
             best[at, :k] = s
-            rows[at, :k] = torch.where(torch.isinf(s) & (s < 0), -1, self.rows[int(pairs.cols.offsets[e]) + i])
+            rows[at, :k] = torch.where(torch.isinf(s) & (s < 0), -1, enrolled[int(pairs.cols.offsets[e]) + i])
         return (rows, best) if is_dev else (rows.cpu().numpy(), best.cpu().numpy().astype(float_cpu(), copy=False))
