@@ -4,23 +4,30 @@
 // hyperion/transforms/cent_whiten.py:25-33, lda.py:31-34, pca.py:39-42, lnorm.py:14-17 whose parameters
 // depend on the row's group).
 //
-// Arithmetic.  Both operands are written as sums of two fp16 numbers, x = 2^-u (x0 + x1) with one power of
-// two per row, w = 2^-v (w0 + w1) with one per output column, and
-//     x w ~= 2^-(u + v) (x0 w0 + x0 w1 + x1 w0)
+// Arithmetic.  Both operands are written as sums of two fp16 numbers, x = 2^-u (x0 + 2^-11 x1) with one power of
+// two per row, w = 2^-v (w0 + 2^-11 w1) with one per output column, and
+//     x w ~= 2^-(u + v) (x0 w0 + 2^-11 (x0 w1 + x1 w0))
 // is accumulated in fp32 by v_mfma_f32_16x16x32_f16: the dropped product is 2^-22 |x w|, and a sum over d
-// coordinates has d / 32 times three roundings instead of d.  Vectors that come as fp16 or bf16 are exact in
-// x0 and take two products.  Against fp32 matrix instructions this is a third to a half of the issue time
-// of the same product.
+// coordinates has d / 32 times four roundings instead of d.  The bracket is summed over the 32 coordinates of one
+// instruction and added to the rest by a fused multiply-add.  The second numbers have the range of the first: written
+// without the 2^11 they end 2^-33 below a row's largest magnitude, and a whitening whose coordinates span six decades
+// comes out at 1.5e-5 instead of 1e-7.  Against fp32 matrix instructions this is a third to a half of the issue time of
+// the same product.
 //
 // A row's scale has to be known before its first value is written, and the row is read once: the scale is
-// taken from the chunk of coordinates at hand (largest magnitude to [2^8, 2^9)), kept while later chunks stay
-// below 2^15, and lowered otherwise, with the sums so far multiplied by the (exact) power of two.  Six
-// powers of two of headroom cost nothing: x1 keeps 2^-33 of the row's largest magnitude.
+// taken from the chunk of coordinates at hand, kept while later chunks stay below 2^15, and lowered otherwise, with the
+// sums so far multiplied by the (exact) power of two.  The largest magnitude goes to [2^14, 2^15) where a row is one
+// chunk, and to [2^8, 2^9) where it may still grow: a coordinate is held to 22 bits, or to 2^-36 of the scaled unit.
 //
-// Measured: 127 500 fp32 rows of 24 groups, 512 -> 150, 96 us (3.6 TB/s; the copy of as much 69); 115 700 bf16 rows of
-// 6 groups by an order, 512 -> 200, 97 us (2.2 TB/s; without the memory 68, without the products 88, without the
-// stores 94: the steps of a workgroup overlap only in part); 19 200 rows of 200 groups, 200 -> 77, normalised 13.4 us;
-// 12 rows of 8 groups, 512 -> 200, 9.0 us, the latency of table, row number, row and norm one after the other.
+// fp16 rows are exact in x0 and take two products: their scale is never below one, so that no value is lost.  bf16 rows
+// are exact in x0 as well unless a value lies below 2^-17 of the scaled unit; a chunk says so when it is written, and
+// only then takes the third product.
+//
+// Measured: 127 500 fp32 rows of 24 groups, 512 -> 150, 104 us (3.3 TB/s; the copy of as much 69); 115 700 bf16 rows of
+// 6 groups by an order, 512 -> 200, 106 us (2.0 TB/s); 19 200 rows of 200 groups, 200 -> 77, normalised 13.5 us; 12 rows
+// of 8 groups, 512 -> 200, 9.1 us, the latency of table, row number, row and norm one after the other.  The multiply-adds
+// that the scaled second numbers need are 64 of a wave's instructions per k-step of a 128-row tile beside 48 products (32
+// where rows have 16 bits): the first two cases take 100 and 95 us without them, with the accuracy lost.
 #include "grouped.h"
 
 #include <type_traits>
@@ -58,6 +65,17 @@ struct Load4<__bf16> {
 
 constexpr int AFFINE_RUN = 8;  // tiles dealt to an XCD at a time
 
+// x up -> x0 + 2^-11 x1 with x0 = fp16(x up), x1 = fp16(2^11 (x up - x0)), four values and a power of two `up`:
+// |x up - x0 - 2^-11 x1| <= 2^-22 |x up| + 2^-36.  An infinity becomes (inf, NaN): its products are NaN.
+__device__ __forceinline__ void split_wide4(f32x4 x, float up, f16x4& x0, f16x4& x1) {
+    const f32x4 t = x * up;
+    x0 = __builtin_convertvector(t, f16x4);
+    f32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fmaf((float)x0[i], -2048.f, t[i] * 2048.f);
+    x1 = __builtin_convertvector(r, f16x4);
+}
+
 struct AffineArgs {
     const void* x;
     int64_t ldx;
@@ -78,8 +96,9 @@ struct AffineArgs {
 };
 
 // RT row tiles of 16 per workgroup of eight waves, which take two column tiles of 16 each.  Coordinates are taken in
-// chunks: 32 for RT = 8, where many workgroups follow one another, up to 1024 / RT for the small tiles, where a row is
-// usually one chunk and everything it needs is requested at once.  The chunk at hand sits in
+// chunks: 32 for RT = 8, 64 for RT = 4 (128 and 256 do not fit the registers of four waves per SIMD: 512 -> 200 with
+// 128 rows a group 31 us with 64, 33 with 128, 79 with 256), 1024 for RT = 1, where a row is usually one chunk and
+// everything it needs is requested at once.  The chunk at hand sits in
 // LDS as pairs in operand order (lane l of a 16 x 32 tile: row l & 15, coordinates 8 (l >> 4) .. + 7; the row is
 // XORed with 4 (l >> 4) so that the four coordinate groups of a row fall into different banks when they are written),
 // the next one is on its way in registers.  Memory operations of a wave complete in order, so the weights of a whole
@@ -89,8 +108,9 @@ template <typename XT, int RT>
 __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(AffineArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int TM = 16 * RT;
-    constexpr int KC = RT == 8 ? 32 : 1024 / RT;
-    constexpr int NP = sizeof(XT) == 4 ? 2 : 1;  // parts of x
+    constexpr int KC = RT == 8 ? 32 : RT == 4 ? 64 : 1024;
+    constexpr bool F16 = std::is_same<XT, _Float16>::value, BF16 = std::is_same<XT, __bf16>::value;
+    constexpr int NP = F16 ? 1 : 2;              // parts of x
     constexpr int LPR = RT == 1 ? 32 : 8;        // lanes that load one row
     constexpr int RPT = TM * LPR / 512;          // rows per thread
     constexpr int F4 = KC / (4 * LPR);           // groups of four coordinates per thread and row
@@ -100,6 +120,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     constexpr int BUF = KSC * RT * NP * 64;
     __shared__ int exps[3][TM];  // a chunk's scales are still read while those of the next but one are written
     __shared__ int lowered[2];  // the chunk for which a scale was lowered last, by buffer
+    __shared__ int second[2];   // the chunk in which an x1 was not zero last (bf16)
     __shared__ int rows[TM];
     __shared__ double norm[CW][TM];
 
@@ -119,6 +140,8 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
 
     // ---- loading side: this thread's rows and coordinates
     const int c = tid % LPR, rg = tid / LPR;
+    const int chunks = (g.d_in + KC - 1) / KC;
+    const int top_exp = chunks == 1 ? 15 : 9;
     int run[RPT];
     f32x4 v[RPT][F4];
 #pragma unroll
@@ -151,8 +174,9 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
             m = dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(m)));
             if (LPR == 32) m = swap16_max(dpp_max<0x140>(m));
             const int ex = __builtin_amdgcn_frexp_expf(m);
-            if (m > 0.f && ex + run[i] > 15) {
-                run[i] = 9 - ex;
+            if (m > 0.f && ex + run[i] > 15 && (!F16 || run[i] > 0)) {
+                run[i] = top_exp - ex;
+                if (F16 && run[i] < 0) run[i] = 0;
                 lowered[buf] = ch;
             }
             const float up = exp2_int(run[i]);
@@ -165,7 +189,11 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
                 if (F4 > 1 && ch * KC + 4 * LPR * f >= 32 * g.ks) break;
                 const int s = k >> 5, kq = (k >> 3) & 3, half = (k >> 2) & 1;
                 f16x4 x0, x1;
-                split_pair4(v[i][f], up, x0, x1);
+                split_wide4(v[i][f], up, x0, x1);
+                if (BF16) {
+                    const uint2 b = __builtin_bit_cast(uint2, x1);
+                    if (b.x | b.y) second[buf] = ch;
+                }
                 f16x4* dst = reinterpret_cast<f16x4*>(
                                  &tile_mem[buf * BUF + ((s * RT + rt) * NP) * 64 + kq * 16 + (r16 ^ (4 * kq))]) + half;
                 dst[0] = x0;
@@ -187,7 +215,6 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const int chunks = (g.d_in + KC - 1) / KC;
 
     // the chunk loop of a wave with `tiles` column tiles
     auto walk = [&](auto tiles_tag) {
@@ -206,23 +233,60 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
                 w[slot][j][1] = __builtin_bit_cast(f16x8, p[64]);
             }
         };
-        auto step = [&](int buf, int slot, int s) {
+        auto step = [&](int buf, int slot, int s, bool third) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 const uint4* xp = &tile_mem[buf * BUF + ((s * RT + i) * NP) * 64 + xs];
                 const f16x8 x0 = __builtin_bit_cast(f16x8, xp[0]);
+                f32x4 low[N > 0 ? N : 1];  // the products of order 2^-11
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][1], x0, acc[i][j], 0, 0, 0);
-                if constexpr (NP == 2) {
+                    low[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][1], x0, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                if constexpr (NP == 2 && !BF16) {
                     const f16x8 x1 = __builtin_bit_cast(f16x8, xp[64]);
 #pragma unroll
                     for (int j = 0; j < N; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x1, acc[i][j], 0, 0, 0);
+                        low[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x1, low[j], 0, 0, 0);
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x0, acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(low[j][q], 0x1p-11f, acc[i][j][q]);
+            }
+            if (BF16 && third) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const f16x8 x1 = __builtin_bit_cast(f16x8, tile_mem[buf * BUF + ((s * RT + i) * NP + 1) * 64 + xs]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const f32x4 low = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[slot][j][0], x1,
+                                                                                 (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(low[q], 0x1p-11f, acc[i][j][q]);
+                    }
+                }
+            }
+        };
+        // the k-steps of chunk `ch`
+        auto multiply = [&](int buf, int ch) {
+            const bool third = BF16 && __builtin_amdgcn_readfirstlane(second[buf]) == ch;
+            if constexpr (KSC == WS) {
+#pragma unroll
+                for (int s = 0; s < KSC; ++s)
+                    if (ch * KSC + s < g.ks) step(buf, s, s, third);
+            } else {
+                // a long chunk: the weights go round a ring of WS k-steps
+                for (int s0 = 0; s0 < KSC; s0 += WS) {
+                    if (ch * KSC + s0 >= g.ks) break;
+#pragma unroll
+                    for (int s = 0; s < WS; ++s) {
+                        if (ch * KSC + s0 + s < g.ks) step(buf, s, s0 + s, third);
+                        weights(s, ch * KSC + s0 + s + WS);
+                    }
+                }
             }
         };
         fetch(0);  // first: converting the rows waits for nothing else
@@ -247,21 +311,7 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
                             for (int q = 0; q < 4; ++q) acc[i][j][q] = ldexpf(acc[i][j][q], by);
                     }
                 }
-                if constexpr (KSC == WS) {
-#pragma unroll
-                    for (int s = 0; s < KSC; ++s)
-                        if (ch * KSC + s < g.ks) step(buf, s, s);
-                } else {
-                    // a long chunk: the weights go round a ring of WS k-steps
-                    for (int s0 = 0; s0 < KSC; s0 += WS) {
-                        if (ch * KSC + s0 >= g.ks) break;
-#pragma unroll
-                        for (int s = 0; s < WS; ++s) {
-                            if (ch * KSC + s0 + s < g.ks) step(buf, s, s0 + s);
-                            weights(s, ch * KSC + s0 + s + WS);
-                        }
-                    }
-                }
+                multiply(buf, ch);
             }
             if (ch + 1 < chunks) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -384,7 +434,7 @@ __global__ __launch_bounds__(256) void grouped_weights_kernel(const float* __res
             const int k = 8 * kb + q;
             const float x = (cc < d_out && k < d_in) ? ldexpf(src[(int64_t)k * d_out], up) : 0.f;
             p0[q] = (_Float16)x;
-            p1[q] = (_Float16)(x - (float)p0[q]);
+            p1[q] = (_Float16)((x - (float)p0[q]) * 2048.f);
         }
         uint4* dst = out + (kb >> 2) * 128 + (kb & 3) * 16 + c;
         dst[0] = __builtin_bit_cast(uint4, p0);
@@ -452,8 +502,8 @@ int launch_affine(const AffineArgs& g, hipStream_t stream) {
     const int per = 16;  // column tiles of a workgroup
     const int64_t gx = xcd_grid(g.n_tiles, AFFINE_RUN), gy = (g.ct + per - 1) / per;
     HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
-    constexpr int KC = RT == 8 ? 32 : 1024 / RT;
-    const int lds = (g.d_in > KC ? 2 : 1) * KC * 16 * RT * (sizeof(XT) == 4 ? 4 : 2);
+    constexpr int KC = RT == 8 ? 32 : RT == 4 ? 64 : 1024;
+    const int lds = (g.d_in > KC ? 2 : 1) * KC * 16 * RT * (std::is_same<XT, _Float16>::value ? 2 : 4);
     if (lds > 48 * 1024)
         HYPMI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&grouped_affine_kernel<XT, RT>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds));

@@ -17,16 +17,17 @@ _AFFINE_TILES = (16, 64, 128)
 _Q4_TESTS = (16, 32, 64)
 
 
-def _affine_tile(mean, d_in, d_out, itemsize):
+def _affine_tile(mean, d_in, itemsize):
     """Rows per workgroup of the affine map, by the mean size of the groups.  Measured with 200 groups of ragged
-    sizes, tiles of 16 / 64 / 128 rows in us: fp32 200 -> 200 with 22 rows a group 15.5 / 16.7 / 18.6, with 37 rows
-    21.8 / 17.6 / 19.6, with 117 rows 46 / 23.5 / 26, with 195 rows 64 / 37 / 28.5.  fp32 rows that do not fit one
-    chunk of the tile of 64 (256 coordinates) keep two of 64 KB in shared memory, one workgroup per CU, which pays
-    only with few columns to multiply them with: 512 -> 200 with 64 rows 66 / 67 / 48, 512 -> 77 with 83 rows
-    29 / 23 / 27."""
+    sizes, tiles of 16 / 64 / 128 rows in us.  Small groups: fp32 200 -> 200 with 12 rows a group 10.7 / 12.4 / 18,
+    with 24 rows 15.2 / 13.3 / 19; 512 -> 200 18.6 / 20.6 / 33 and 22.4 / 21.3 / 33.  Large ones, tiles of 64 / 128:
+    fp32 512 -> 200 with 200 rows 44 / 50, with 870 rows 42 / 49; 512 -> 150 with 5600 rows 144 / 160; 96 -> 64 with
+    32 000 rows 20.5 / 19.3, which has few coordinates to overlap with what starts and ends a tile.  Rows of 16 bits
+    are less work to convert and take the larger tile, which reads the weights half as often: bf16 512 -> 150 with 400 rows
+    76 / 90, with 1500 rows 59 / 56; 512 -> 200 with 19 000 rows 114 / 107."""
     if mean <= 20:
         return 16
-    return 64 if mean <= 140 and (itemsize == 2 or d_in <= 256 or d_out <= 128) else 128
+    return 128 if mean > 1000 and (itemsize == 2 or d_in <= 128) else 64
 
 
 def _prefix(counts):
@@ -229,7 +230,7 @@ class GroupPairs(_Plan):
 
 class AffineBank(_Plan):
     """One affine map per group, x -> x W[e] + b[e], laid out for grouped_affine.  W [E, d_in, d_out] and b
-    [E, d_out] (or None), host arrays or device tensors of any float type, kept at fp32 accuracy.  dims
+    [E, d_out] (or None), host arrays or device tensors of any float type, taken as fp32.  dims
     [E] (optional): dimension of every map where they differ; W[e][:, dims[e]:] and b[e][dims[e]:] have to be
     zero, and the length normalisation scales to sqrt(dims[e]).  The maps are laid out by the time the constructor
     returns, so that any stream can use them at once; made while a HIP graph is captured they are part of the graph."""
@@ -310,7 +311,9 @@ def _device_rows(x, types, what):
 def grouped_affine(x, groups, bank, lnorm=False, out=None):
     """y_r = x_r W_e + b_e for every row r of group e, with lnorm followed by the length normalisation
     y <- sqrt(dim_e) y / (|y| + 1e-10).  x: device fp32, fp16 or bf16 [n, d_in]; returns device fp32
-    [n, d_out] (fp32 accuracy).  With an ordered RowGroups row i of the result belongs to row i of x; rows of
+    [n, d_out].  The coordinates of a row count to 22 bits, or to 2^-42 of the largest magnitude of their row where
+    that is more (fp16 rows are taken exactly), weights to 22 bits or 2^-48 of the largest of their column; sums are
+    fp32.  With an ordered RowGroups row i of the result belongs to row i of x; rows of
     no group are zero in a new result and left alone in `out` (fp32, 16-byte aligned rows, also a view whose
     storage goes on behind a row)."""
     torch = _torch()
@@ -335,7 +338,7 @@ def grouped_affine(x, groups, bank, lnorm=False, out=None):
             raise ValueError("out must be fp32 [%d, %d] on %s with 16-byte aligned rows" % (n, d, x.device))
         if _overlap(x, y):
             raise ValueError("out must not share memory with x")
-    tile = _affine_tile(groups._mean, bank.d_in, d, x.element_size())
+    tile = _affine_tile(groups._mean, bank.d_in, x.element_size())
     n_tiles = groups._n_tiles[tile]
     if n_tiles:
         _run(_lib.load().hypmi_grouped_affine, x.device, (groups, bank), x.data_ptr(), kinds[x.dtype], ldx, bank.d_in,

@@ -551,9 +551,12 @@ int hypmi_grouped_weights(const float* W, const float* b, int n_groups, int d_in
  * aligned, ldy a multiple of 4 and at least d_out; cols_y columns of a row are written, d_out or up to the next multiple of 4 (zeros
  * behind d_out, so that rows which follow one another leave no gaps in the lines that are written); what lies
  * behind them and rows of no group are left as they are.  With `order` row order[i] of x goes to row order[i] of y; no
- * row may occur twice.  tiles: prefix sums of ceil(size / tile_rows), tile_rows 16, 64 or 128.  Accurate to
- * fp32 (fp16-pair products, fp32 accumulation); a row with a NaN or an infinity comes out
- * without finite values (fp32 rows: as NaN). */
+ * row may occur twice.  tiles: prefix sums of ceil(size / tile_rows), tile_rows 16, 64 or 128.  Accuracy: a coordinate
+ * counts to 22 bits, or to 2^-42 of the largest magnitude of its row where that is more (fp16 rows exactly), a weight to
+ * 22 bits or to 2^-48 of the largest of its column, sums are fp32:
+ *   |error of y_rj| <= (3 + d_in) 2^-22 sum_k |x_rk w_kj| + 2^-42 max_k |x_rk| sum_k |w_kj|
+ *                      + 2^-48 max_k |w_kj| sum_k |x_rk|.
+ * A row with a NaN or an infinity comes out without finite values (fp32 rows: as NaN). */
 int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int d_in, const int64_t* offsets,
                          const int64_t* tiles, int tile_rows, int n_groups, int64_t n_rows, int64_t n_tiles,
                          const int32_t* order, const void* weights, const void* columns, const int32_t* dims,
