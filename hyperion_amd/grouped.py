@@ -255,6 +255,9 @@ class AffineBank(_Plan):
                     (dims.size and (dims.min() < 1 or dims.max() > self.d_out)):
                 raise ValueError("dims must be %d integers in 1 .. %d" % (self.num_groups, self.d_out))
             self.dims = torch.from_numpy(dims.astype(np.int32)).to(self.device)
+            used = (W != 0).any(1) if b is None else (W != 0).any(1) | (b != 0)
+            if bool((used & (torch.arange(self.d_out, device=self.device) >= self.dims[:, None])).any()):
+                raise ValueError("W and b must be zero behind dims: those columns would enter the length normalisation")
         lib = _lib.load()
         args = (self.num_groups, self.d_in, self.d_out)
         self._w = torch.empty(lib.hypmi_grouped_weights_bytes(*args) // 4, dtype=torch.int32, device=self.device)

@@ -546,7 +546,8 @@ int hypmi_grouped_weights(const float* W, const float* b, int n_groups, int d_in
                           void* columns, void* stream);
 
 /* y_r = x_r W_e + b_e for every row r of every group e, and with lnorm != 0 then
- * y_r <- sqrt(dims[e]) y_r / (|y_r| + 1e-10)  (dims NULL: d_out).  x: rows of d_in elements of x_type
+ * y_r <- sqrt(dims[e]) y_r / (|y_r| + 1e-10)  (dims NULL: d_out; otherwise the columns of W and b behind dims[e]
+ * have to be zero, they enter the norm).  x: rows of d_in elements of x_type
  * (HYPMI_F32, HYPMI_F16 or HYPMI_BF16), ldx >= d_in, any alignment of the element type.  y: fp32, 16-byte
  * aligned, ldy a multiple of 4 and at least d_out; cols_y columns of a row are written, d_out or up to the next multiple of 4 (zeros
  * behind d_out, so that rows which follow one another leave no gaps in the lines that are written); what lies

@@ -125,3 +125,22 @@ def test_rows_that_grow_and_shrink_from_chunk_to_chunk():
                     bound, _ = _bound(xs[at:at + k], W[g].astype(float))
                     assert (np.abs(y[at:at + k] - want) <= bound + 2 * U * (np.abs(want) + np.abs(b[g]))).all()
                 at += k
+
+
+def test_columns_behind_the_dimension_of_a_map_are_refused():
+    """They would enter the length normalisation and be written where zeros are promised."""
+    from hyperion_amd import engine
+
+    W, b = np.ones((3, 5, 8)), np.ones((3, 8))
+    dims = [8, 2, 5]
+    for e, k in enumerate(dims):
+        W[e, :, k:], b[e, k:] = 0, 0
+    engine.AffineBank(W, b, dims=dims)
+    engine.AffineBank(W, dims=dims)
+    for bad in (1e-30, np.nan, np.inf):
+        for array, at in ((W, (1, 4, 2)), (W, (2, 0, 7)), (b, (1, 7))):
+            array[at] = bad
+            with pytest.raises(ValueError, match="behind dims"):
+                engine.AffineBank(W, b, dims=dims)
+            array[at] = 0
+    engine.AffineBank(W, b, dims=dims)
