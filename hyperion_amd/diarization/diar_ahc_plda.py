@@ -125,10 +125,11 @@ class DiarAHCPLDA:
 
     def scores_batch(self, xs):
         """Self-score matrices of a batch of recordings, each [segments, dim]: a list of device tensors
-        [n, n], views of one buffer.  The steps of `scores` (without its float64 refinement: entries that cancel
+        [n, n].  The steps of `scores` (without its float64 refinement: entries that cancel
         to about zero carry an absolute error of some 1e-6 of the terms they are the difference of), every step
         one launch over all recordings: moments, projection with length normalisation, model basis, packing and
-        the blocks of scores.  A recording needs two segments where a PCA is fitted on it."""
+        the blocks of scores (one launch per recording above 510 latent dimensions, where packed rows are wider than
+        the grouped product takes).  A recording needs two segments where a PCA is fitted on it."""
         torch = engine.require_gpu()
         xs = [engine.upload(x) for x in xs]
         if not xs:
@@ -153,6 +154,9 @@ class DiarAHCPLDA:
         else:
             plan = self.plda_model.score_plan()
             G1, G2 = plan.prologue(x, engine.SIDE_ENROL), plan.prologue(x, engine.SIDE_TEST)
+        if not engine.grouped_score_supported(G1.shape[1]):
+            at = groups.offsets
+            return [engine.score(G1[a:b], G2[a:b]) for a, b in zip(at[:-1], at[1:])]
         return pairs.blocks(engine.grouped_score(G1, G2, pairs))
 
     def cluster_batch(self, xs):

@@ -615,7 +615,7 @@ def to_host(t, dtype):
 
 
 _GROUPED = ("AffineBank", "GroupPairs", "Q4Rows", "RowGroups", "grouped_affine", "grouped_gram64", "grouped_pack",
-            "grouped_score", "q4_rows", "q4_score")
+            "grouped_score", "grouped_score_supported", "q4_rows", "q4_score")
 
 
 def __getattr__(name):

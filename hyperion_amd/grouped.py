@@ -395,6 +395,11 @@ def grouped_pack(s, groups, maps, c, sides="both"):
     return G1, G2
 
 
+def grouped_score_supported(kp):
+    """Whether grouped_score takes packed rows of kp elements (multiples of 8 up to 512)."""
+    return bool(_lib.load().hypmi_grouped_score_rows(int(kp)))
+
+
 def grouped_score(G1, G2, pairs, out=None):
     """Scores of packed enrol rows against packed test rows of the same group (Plan.prologue, both [n, kp]):
     the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e)."""
