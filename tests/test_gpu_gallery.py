@@ -36,3 +36,56 @@ def test_gallery_is_written_when_enrol_returns():
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and keep.shape == (4096, 4096)
     assert g.gallery.k == 20 and g.rows.shape == (100,)
+
+
+def _gallery(n, partitions=None, seed=3):
+    """A gallery of n random vectors of a small model, and that model."""
+    import numpy as np
+
+    import synth
+    from hyperion_amd.gallery import PLDAGallery
+    from hyperion_amd.pdfs.plda import SPLDA
+
+    m = synth.make_splda(24, 12)
+    x = np.random.RandomState(seed).randn(n, 24).astype(np.float32)
+    part = None if partitions is None else np.random.RandomState(seed + 1).randint(0, partitions, n)
+    return PLDAGallery(SPLDA(mu=m["mu"], V=m["V"], W=m["W"])).enrol(x, part, partitions)
+
+
+@pytest.mark.parametrize("partitions", [None, 5])
+@pytest.mark.parametrize("scores", [1, 150, 1000, 4001])
+def test_identify_in_slices(monkeypatch, scores, partitions):
+    """However few scores fit at a time, down to those of less than one test, the answer is the same."""
+    import numpy as np
+
+    from hyperion_amd import gallery
+
+    g = _gallery(400, partitions)
+    x = np.random.RandomState(9).randn(33, 24)
+    part = None if partitions is None else np.random.RandomState(8).choice([0, 1, 3], 33)
+    want = g.identify(x, 6, part)
+    monkeypatch.setattr(gallery, "_SLICE_BYTES", 4 * scores)
+    got = g.identify(x, 6, part)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def test_identify_holds_few_scores_at_a_time(monkeypatch):
+    """1500 tests against 400 000 rows are 2.4 GB of scores; 1 GiB of them, their mask and some more are held."""
+    import numpy as np
+    import torch
+
+    from hyperion_amd import gallery
+
+    monkeypatch.setattr(gallery, "_SLICE_BYTES", 1 << 30)
+    g = _gallery(400000)
+    x = torch.from_numpy(np.random.RandomState(9).randn(1500, 24)).float().cuda()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    rows, best = g.identify(x, 5)
+    assert torch.cuda.max_memory_allocated() - before < 2 << 30
+    at = [0, 700, 1499]
+    one = [g.identify(x[i:i + 1], 5) for i in at]
+    # whatever is scored together, a score is the same sum in another order of roundings at most: 64 2^-24 of its terms
+    for i, (r, b) in zip(at, one):
+        assert torch.equal(r[0], rows[i]) and torch.allclose(b[0], best[i], rtol=1e-5, atol=1e-4)
