@@ -292,7 +292,7 @@ __global__ __launch_bounds__(256, TT == 4 ? 2 : 3) void q4_score_kernel(Q4Args g
 template <int KH, int TT>
 int launch_q4(const Q4Args& g, hipStream_t stream) {
     const int64_t grid = xcd_grid(g.n_tasks, Q4_RUN);
-    HYPMI_REQUIRE(grid <= 0x7fffffffLL, "q4_score: too many workgroups");
+    HYPMI_REQUIRE(fits_launch(grid, 256), "q4_score: too many workgroups");
     const int lds = TT * KH * g.phases * 2048;
     if (lds > 48 * 1024)
         HYPMI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_score_kernel<KH, TT>),
@@ -334,7 +334,7 @@ extern "C" int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* 
     HYPMI_REQUIRE(G && offsets && blocks && codes && scales && q, "q4_rows: null pointer");
     HYPMI_REQUIRE(aligned16(codes) && aligned16(scales), "q4_rows: buffers must be 16-byte aligned");
     const int64_t grid = (n_blocks * ks + 3) / 4;
-    HYPMI_REQUIRE(grid <= 0x7fffffffLL, "q4_rows: too many rows");
+    HYPMI_REQUIRE(fits_launch(grid, 256), "q4_rows: too many rows");
     hipLaunchKernelGGL(q4_rows_kernel, dim3((unsigned)grid), dim3(256), 0, stream, G, ldg, k, ks, offsets, blocks,
                        n_groups, n_blocks, static_cast<unsigned*>(codes), static_cast<unsigned short*>(scales), q);
     HYPMI_HIP(hipGetLastError());

@@ -36,6 +36,9 @@ __device__ __forceinline__ int64_t xcd_task(int64_t b, int64_t n, int run) {
     return t < n ? t : -1;
 }
 
+// A launch holds fewer than 2^32 work-items in a dimension.
+inline bool fits_launch(int64_t blocks, int threads) { return blocks >= 0 && blocks <= 0xffffffffLL / threads; }
+
 inline int64_t xcd_grid(int64_t n, int run) { return (n + 8 * run - 1) / (8 * run) * (8 * run); }
 
 // 2^e as a float, -126 <= e <= 127

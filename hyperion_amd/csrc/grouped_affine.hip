@@ -443,65 +443,68 @@ __global__ __launch_bounds__(256) void grouped_weights_kernel(const float* __res
 }
 
 // Length normalisation of rows of y by group where a row does not fit one workgroup of the product
-// (more than 256 output columns): one wave per listed row.
+// (more than 256 output columns): a wave per listed row, the rows in turn.
 __global__ __launch_bounds__(256) void grouped_lnorm_kernel(float* __restrict__ y, int64_t ldy, int d_out,
                                                             const int64_t* __restrict__ offsets, int n_groups,
                                                             const int32_t* __restrict__ order,
                                                             const int32_t* __restrict__ dims, int64_t n) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= n) return;
     const int lane = threadIdx.x & 63;
-    double top = (double)d_out;
-    if (dims) top = (double)dims[find_group(offsets, n_groups, r)];
-    float* row = y + (order ? (int64_t)order[r] : r) * ldy;
-    double s = 0.0;
-    for (int k = lane; k < d_out; k += 64) s = fma((double)row[k], (double)row[k], s);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4) {
+        double top = (double)d_out;
+        if (dims) top = (double)dims[find_group(offsets, n_groups, r)];
+        float* row = y + (order ? (int64_t)order[r] : r) * ldy;
+        double s = 0.0;
+        for (int k = lane; k < d_out; k += 64) s = fma((double)row[k], (double)row[k], s);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    const float f = (float)(sqrt(top) / (sqrt(s) + 1e-10));
-    for (int k = lane; k < d_out; k += 64) row[k] *= f;
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        const float f = (float)(sqrt(top) / (sqrt(s) + 1e-10));
+        for (int k = lane; k < d_out; k += 64) row[k] *= f;
+    }
 }
 
 // Packing of projected rows by the maps of their group: g_k = (s_k + shift_t[k]) scale_t[k],
 // h_k = (s_k + shift_n[k]) scale_n[k], q = (|g|^2 - |h|^2) / 2 into an enrol-side row [g, q, 1] and a test-side row
-// [g, 1, q + c] (book_pack_kernel's arithmetic with maps [n_groups][4][K] and constants c[n_groups]).  One wave per
-// row; either side may be left out.
+// [g, 1, q + c] (book_pack_kernel's arithmetic with maps [n_groups][4][K] and constants c[n_groups]).  A wave per
+// row, the rows in turn; either side may be left out.
 __global__ __launch_bounds__(256) void grouped_pack_kernel(const float* __restrict__ s, int64_t lds, int K,
                                                            const int64_t* __restrict__ offsets, int n_groups,
                                                            int64_t n, const float* __restrict__ maps,
                                                            const float* __restrict__ c, float* __restrict__ G1,
                                                            float* __restrict__ G2, int kp) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= n) return;
     const int lane = threadIdx.x & 63;
-    const int e = find_group(offsets, n_groups, r);
-    const float* m = maps + (int64_t)e * 4 * K;
-    const float* row = s + r * lds;
-    float* out1 = G1 ? G1 + r * kp : nullptr;
-    float* out2 = G2 ? G2 + r * kp : nullptr;
-    float sum = 0.f;
-    for (int k = lane; k < K; k += 64) {
-        const float v = row[k];
-        const float g = (v + m[k]) * m[K + k], h = (v + m[2 * K + k]) * m[3 * K + k];
-        sum += (g - h) * (g + h);
-        if (out1) out1[k] = g;
-        if (out2) out2[k] = g;
-    }
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4) {
+        const int e = find_group(offsets, n_groups, r);
+        const float* m = maps + (int64_t)e * 4 * K;
+        const float* row = s + r * lds;
+        float* out1 = G1 ? G1 + r * kp : nullptr;
+        float* out2 = G2 ? G2 + r * kp : nullptr;
+        float sum = 0.f;
+        for (int k = lane; k < K; k += 64) {
+            const float v = row[k];
+            const float g = (v + m[k]) * m[K + k], h = (v + m[2 * K + k]) * m[3 * K + k];
+            sum += (g - h) * (g + h);
+            if (out1) out1[k] = g;
+            if (out2) out2[k] = g;
+        }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    const float q = 0.5f * sum;
-    for (int k = K + lane; k < kp; k += 64) {
-        const int j = k - K;
-        if (out1) out1[k] = j == 0 ? q : j == 1 ? 1.f : 0.f;
-        if (out2) out2[k] = j == 0 ? 1.f : j == 1 ? q + c[e] : 0.f;
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        const float q = 0.5f * sum;
+        for (int k = K + lane; k < kp; k += 64) {
+            const int j = k - K;
+            if (out1) out1[k] = j == 0 ? q : j == 1 ? 1.f : 0.f;
+            if (out2) out2[k] = j == 0 ? 1.f : j == 1 ? q + c[e] : 0.f;
+        }
     }
 }
+
+// Workgroups of four waves that take the rows in turn: 32 for each of 256 CUs at most
+inline unsigned row_blocks(int64_t n) { return (unsigned)(n < 4 * 8192 ? (n + 3) / 4 : 8192); }
 
 template <typename XT, int RT>
 int launch_affine(const AffineArgs& g, hipStream_t stream) {
     const int per = 16;  // column tiles of a workgroup
     const int64_t gx = xcd_grid(g.n_tiles, AFFINE_RUN), gy = (g.ct + per - 1) / per;
-    HYPMI_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, "grouped_affine: too many workgroups");
+    HYPMI_REQUIRE(fits_launch(gx, 512) && gy <= 65535, "grouped_affine: too many workgroups");
     constexpr int KC = RT == 8 ? 32 : RT == 4 ? 64 : 1024;
     const int lds = (g.d_in > KC ? 2 : 1) * KC * 16 * RT * (std::is_same<XT, _Float16>::value ? 2 : 4);
     if (lds > 48 * 1024)
@@ -544,7 +547,7 @@ extern "C" int hypmi_grouped_weights(const float* W, const float* b, int n_group
     HYPMI_REQUIRE(aligned16(w) && aligned16(columns), "grouped_weights: buffers must be 16-byte aligned");
     const int ct = (d_out + 15) / 16, ks = (d_in + 31) / 32;
     const int64_t blocks = (int64_t)n_groups * ct;
-    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_weights: too many groups");
+    HYPMI_REQUIRE(fits_launch(blocks, 256), "grouped_weights: too many groups");
     hipLaunchKernelGGL(grouped_weights_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, W, b, d_in, d_out, ct, ks,
                        static_cast<uint4*>(w), static_cast<float*>(columns));
     HYPMI_HIP(hipGetLastError());
@@ -578,9 +581,7 @@ extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int 
         default: rc = launch_affine_type<__bf16>(g, tile_rows, stream); break;
     }
     if (rc != HYPMI_OK || !lnorm || fused) return rc;
-    const int64_t blocks = (n_rows + 3) / 4;
-    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_affine: too many rows");
-    hipLaunchKernelGGL(grouped_lnorm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, y, ldy, d_out, offsets,
+    hipLaunchKernelGGL(grouped_lnorm_kernel, dim3(row_blocks(n_rows)), dim3(256), 0, stream, y, ldy, d_out, offsets,
                        n_groups, order, dims, n_rows);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
@@ -593,9 +594,7 @@ extern "C" int hypmi_grouped_pack(const float* s, int64_t lds, int K, const int6
     HYPMI_REQUIRE(G1 || G2, "grouped_pack: no result asked for");
     if (n_rows == 0) return HYPMI_OK;
     HYPMI_REQUIRE(s && offsets && maps && c, "grouped_pack: null pointer");
-    const int64_t blocks = (n_rows + 3) / 4;
-    HYPMI_REQUIRE(blocks <= 0x7fffffffLL, "grouped_pack: too many rows");
-    hipLaunchKernelGGL(grouped_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, s, lds, K, offsets, n_groups,
+    hipLaunchKernelGGL(grouped_pack_kernel, dim3(row_blocks(n_rows)), dim3(256), 0, stream, s, lds, K, offsets, n_groups,
                        n_rows, maps, c, G1, G2, kp);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;

@@ -323,9 +323,10 @@ extern "C" int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, in
     double* part = static_cast<double*>(workspace);
     const GramArgs g = {x, ldx, d, w, offsets, units, slots, n_groups, n_units, order, C, F, part,
                         part ? part + n_slots * pairs * 1024 : nullptr, nb, pairs};
+    HYPMI_REQUIRE(fits_launch(n_units, 256), "grouped_gram: too many units of work");  // below 2^24: no product overflows
     const int64_t grid = xcd_grid(n_units * ((pairs + 3) / 4), (pairs + 3) / 4);
     const int64_t reduce = n_slots ? (int64_t)n_groups * pairs : 0;
-    HYPMI_REQUIRE(grid <= 0x7fffffffLL && reduce <= 0x7fffffffLL, "grouped_gram: too many workgroups");
+    HYPMI_REQUIRE(fits_launch(grid, 256) && fits_launch(reduce, 256), "grouped_gram: too many workgroups");
     const dim3 blocks((unsigned)grid), threads(256);
     auto launch = [&](auto type, auto ordered) {
         typedef decltype(type) XT;

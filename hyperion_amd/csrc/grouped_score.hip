@@ -225,7 +225,7 @@ template <int KS>
 int launch_score(const ScoreArgs& g, hipStream_t stream) {
     constexpr int RT = KS == 6 ? 2 : 1, NW = KS <= 5 ? 8 : 4;
     const int64_t grid = xcd_grid(g.n_tasks, SCORE_RUN);
-    HYPMI_REQUIRE(grid <= 0x7fffffffLL, "grouped_score: too many workgroups");
+    HYPMI_REQUIRE(fits_launch(grid, 64 * NW + 128), "grouped_score: too many workgroups");
     hipLaunchKernelGGL((grouped_score_kernel<KS, RT, NW>), dim3((unsigned)grid), dim3(64 * NW + 128), 0, stream, g);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;

@@ -144,3 +144,32 @@ def test_columns_behind_the_dimension_of_a_map_are_refused():
                 engine.AffineBank(W, b, dims=dims)
             array[at] = 0
     engine.AffineBank(W, b, dims=dims)
+
+
+def test_more_rows_than_waves_of_a_launch():
+    """The length normalisation of wide rows and the packing take rows in turn: 32 768 are one round."""
+    import torch
+
+    from hyperion_amd import engine
+
+    n, d, m = 70001, 4, 258
+    r = np.random.RandomState(5)
+    sizes = [32767, 0, 2, 37232]
+    x = torch.from_numpy(r.randn(n, d)).float().cuda()
+    W = r.randn(4, d, m).astype(np.float32)
+    groups = engine.RowGroups(sizes)
+    y = engine.grouped_affine(x, groups, engine.AffineBank(W), lnorm=True)
+    plain = engine.grouped_affine(x, groups, engine.AffineBank(W)).double()
+    want = plain * math.sqrt(m) / plain.norm(dim=1, keepdim=True)
+    assert ((y.double() - want).abs() <= 8 * U * want.abs()).all()  # the factor and the product, both rounded
+    s = torch.from_numpy(r.randn(n, 6)).float().cuda()
+    maps, c = r.randn(4, 4, 6).astype(np.float32), r.randn(4).astype(np.float32)
+    G1, G2 = engine.grouped_pack(s, groups, maps, c)
+    at = np.cumsum([0] + sizes)
+    for e in (0, 2, 3):
+        one = engine.RowGroups([sizes[e]])
+        for part in range(at[e], at[e + 1], 20000):  # no more than one round at a time
+            end = min(part + 20000, int(at[e + 1]))
+            one = engine.RowGroups([end - part])
+            for got, want in zip((G1, G2), engine.grouped_pack(s[part:end], one, maps[e:e + 1], c[e:e + 1])):
+                assert torch.equal(got[part:end], want)
