@@ -142,7 +142,8 @@ class RowGroups(_Plan):
     def _set_order(self, order):
         torch = _torch()
         if not isinstance(order, torch.Tensor):
-            order = torch.from_numpy(np.ascontiguousarray(order))
+            order = np.ascontiguousarray(order)
+            order = torch.from_numpy(order if order.size else order.astype(np.int64))  # an empty list has no type
         if order.dim() != 1 or order.dtype not in (torch.int32, torch.int64):
             raise ValueError("order must be a 1-D sequence of integers")
         if order.numel() != self.total:

@@ -173,3 +173,20 @@ def test_more_rows_than_waves_of_a_launch():
             one = engine.RowGroups([end - part])
             for got, want in zip((G1, G2), engine.grouped_pack(s[part:end], one, maps[e:e + 1], c[e:e + 1])):
                 assert torch.equal(got[part:end], want)
+
+
+def test_an_empty_order():
+    import torch
+
+    from hyperion_amd import engine
+
+    x = torch.ones(3, 4, device="cuda")
+    for order in ([], np.zeros(0, int), torch.zeros(0, dtype=torch.int32)):
+        groups = engine.RowGroups([0, 0], order=order)
+        assert (engine.grouped_affine(x, groups, engine.AffineBank(np.ones((2, 4, 5)))) == 0).all()
+        C, F = engine.grouped_gram64(x, groups)
+        assert (C == 0).all() and (F == 0).all()
+    with pytest.raises(ValueError, match="lists 0 rows"):
+        engine.RowGroups([1], order=[])
+    with pytest.raises(ValueError, match="1-D"):
+        engine.RowGroups([0], order=[[]])
