@@ -615,7 +615,8 @@ def to_host(t, dtype):
 
 
 _GROUPED = ("AffineBank", "GroupPairs", "Q4Rows", "RowGroups", "grouped_affine", "grouped_gram64", "grouped_pack",
-            "grouped_score", "grouped_score_supported", "q4_rows", "q4_score")
+            "grouped_score", "grouped_score_supported", "q4_rows", "q4_score",
+            "q4_supported")
 
 
 def __getattr__(name):

@@ -11,8 +11,8 @@ _SLICE_BYTES = 4 << 30  # of scores that identify holds at a time (1000 tests x 
 
 class PLDAGallery:
     """Enrolled vectors as 4-bit rows (engine.q4_rows: 94 bytes a row at y_dim 150, a sixth of the packed fp32 row),
-    scored against test vectors in one pass over them.  plda: an SPLDA, FRPLDA or PLDA model; preproc: a
-    TransformList folded in front of it, as in PLDABackend.
+    scored against test vectors in one pass over them.  plda: an SPLDA, FRPLDA or PLDA model of up to 512 latent
+    dimensions; preproc: a TransformList folded in front of it, as in PLDABackend.
 
     The scores are llr_1vs1 (hyperion/pdfs/plda/splda.py:275-316) with the enrolled projections rounded to 4 bits: a
     score is off by at most half a scale per coordinate times the test's projection, about a tenth of the deviation
@@ -25,6 +25,8 @@ class PLDAGallery:
     def __init__(self, plda, preproc=None):
         self.plda = plda
         self.plan = plda.score_plan(preproc)
+        if not engine.q4_supported(self.plan.k):
+            raise ValueError("a gallery holds models of up to 512 latent dimensions, this one has %d" % self.plan.k)
         # (4-bit rows, device int64: row of the enrolled array that each was made from), replaced together
         self._enrolled = None, None
 
@@ -41,6 +43,8 @@ class PLDAGallery:
         vector's partition, 0 .. num_partitions - 1.  Waits until the gallery is written, so that any stream can search it at
         once.  Returns self."""
         torch = engine.require_gpu()
+        if partition is None and num_partitions not in (None, 1):
+            raise ValueError("%d partitions: say which one every vector belongs to" % num_partitions)
         x = engine.upload(x)
         if partition is None:
             groups, order = engine.RowGroups([x.shape[0]], device=x.device), None

@@ -478,6 +478,11 @@ class Q4Rows(_Plan):
         return v[torch.from_numpy(keep).to(v.device)][:, :self.k].contiguous()
 
 
+def q4_supported(k):
+    """Whether the 4-bit operators take rows of k coordinates (1 to 512)."""
+    return bool(_lib.load().hypmi_q4_ksteps(int(k)))
+
+
 def q4_rows(G, k, groups=None):
     """Packed enrol-side rows [g, q, 1] (Plan.prologue; k coordinates) -> Q4Rows.  groups: partitions of the
     gallery (default: one)."""

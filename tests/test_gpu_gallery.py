@@ -89,3 +89,36 @@ def test_identify_holds_few_scores_at_a_time(monkeypatch):
     # whatever is scored together, a score is the same sum in another order of roundings at most: 64 2^-24 of its terms
     for i, (r, b) in zip(at, one):
         assert torch.equal(r[0], rows[i]) and torch.allclose(b[0], best[i], rtol=1e-5, atol=1e-4)
+
+
+def test_refusals():
+    import numpy as np
+
+    import synth
+    from hyperion_amd.gallery import PLDAGallery
+    from hyperion_amd.pdfs.plda import SPLDA
+
+    m = synth.make_splda(516, 513)
+    with pytest.raises(ValueError, match="up to 512 latent dimensions, this one has 513"):
+        PLDAGallery(SPLDA(mu=m["mu"], V=m["V"], W=m["W"]))
+    g = _gallery(10)
+    with pytest.raises(ValueError, match="3 partitions: say which"):
+        g.enrol(np.zeros((4, 24)), num_partitions=3)
+    assert g.enrol(np.ones((4, 24)), num_partitions=1).gallery.groups.num_groups == 1
+
+
+def test_a_gallery_of_512_latent_dimensions():
+    """A score is off by at most half a scale per coordinate times the test's projection, as for smaller models: here
+    the share of its deviation that rounding to 15 levels moves, a fifth."""
+    import numpy as np
+
+    import synth
+    from hyperion_amd.gallery import PLDAGallery
+    from hyperion_amd.pdfs.plda import SPLDA
+
+    m = synth.make_splda(516, 512)
+    plda = SPLDA(mu=m["mu"], V=m["V"], W=m["W"])
+    x = synth.sample_splda(m, 40, 6, seed=7)
+    want = plda.llr_1vs1(x[::2], x[1::2])
+    got = PLDAGallery(plda).enrol(x[::2]).llr(x[1::2])
+    assert np.std(got - want) <= 0.2 * np.std(want)
