@@ -8,18 +8,20 @@
 // are converted here, on their way to the matrix instructions: a block has only as many columns as the group
 // has rows, so a converted copy of the operands would cost as much traffic as the scores themselves.
 //
-// A workgroup has four or eight waves that multiply and two that load.  A multiplying wave keeps 16 RT enrol rows as
+// A workgroup has four or eight waves that multiply and two that load.  A multiplying wave keeps 16 enrol rows as
 // operands in registers and walks up to `span` test rows of its group in tiles of 32 (a group's test rows are cut into
 // equal parts); the loading waves take 16 rows of the next tile each, a row by four lanes, find its largest magnitude,
 // convert it and leave it in LDS in operand order, and request the tile after that.  Memory operations of a wave
 // complete in order, so a wave that both stores scores and loads rows waits for its scores to be written: with four
-// waves that did both, 200 recordings took 42 us instead of 35 and 12 domains 117 instead of 107 at best.  Test rows
+// waves that did both, 200 recordings took 42 us instead of 35; the 12 domains gained little (117 instead of 107 at best
+// for the kernel alone, nothing for passes that follow one another).  Test rows
 // are the first operand of the matrix instruction, so a lane ends up with four neighbouring scores of one enrol row.
 //
-// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 35 us, 12 domains of 300 to
-// 20000 test vectors (68.9 M scores) 105 to 125 us: 2.2 to 2.6 TB/s of results.  The domains write 334 MB for 276 (a
-// row of a block starts anywhere in a line) and read 91 MB for 20, 3.4 TB/s together where a copy reaches 4.95;
-// without the stores they take 95 us, with the stores and one multiplication per span 76 to 85.  Enrol blocks in
+// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 33 to 40 us by the box, 12
+// domains of 300 to 20000 test vectors (68.9 M scores) 136, of which the kernel alone 107 to 126 after a pause: 2.0 TB/s
+// of results.  The domains write 334 MB for 276 (a row of a block starts anywhere in a line) and read 91 MB for 20;
+// without the stores they take 95 us, with the stores and one multiplication per span 76 to 85, so neither alone is the
+// bound: 1152 workgroups, two per CU, are 2.25 rounds, and a loading wave has one tile in flight.  Enrol blocks in
 // turn instead of spans read 47 MB but leave the last workgroups alone for longer (114 us at best); spans of 256 to
 // 1024, 32 rows a wave (109 us), rows converted beforehand by a kernel of their own (131 + 10 us) are not faster.
 #include "grouped.h"
@@ -34,7 +36,7 @@ struct ScoreArgs {
     const int64_t* off1;    // [n_groups + 1]
     const int64_t* off2;
     const int64_t* blocks;  // [n_groups + 1] element offsets of the blocks
-    const int64_t* tasks;   // [n_groups + 1] prefix of ceil(n1 / (64 RT)) * ceil(n2 / span)
+    const int64_t* tasks;   // [n_groups + 1] prefix of ceil(n1 / (16 NW)) * ceil(n2 / span)
     int n_groups;
     int64_t n_tasks;
     int span;
@@ -43,6 +45,12 @@ struct ScoreArgs {
 
 constexpr int SCORE_RUN = 8;     // tasks dealt to an XCD at a time
 constexpr int SCORE_SPAN = 512;  // test rows one workgroup walks at most
+
+// Multiplying waves of a workgroup, 16 enrol rows each.  Recordings (17.5 M scores) / domains (12.5 M) with eight waves, with
+// four, with four that take 32 rows each, in us: 3 k-steps 35 / 23, 39 / 27, 35 / 24; 5 k-steps 40 / 26, 46 / 30,
+// 40 / 27; 6 k-steps 53 / 32, 63 / 39, 62 / 34.  Eight would be faster above 192 columns too (8 k-steps 74 / 39 against
+// 85 / 56, 16 k-steps 144 / 72 against 160 / 103), where callers count their tasks in 64 rows.
+constexpr int score_waves(int ksteps) { return ksteps <= 6 ? 8 : 4; }
 
 // Coordinates 32 s + 8 kq .. + 7 of the row at `p`, s = 0 .. KS - 1; lanes r16 + 16 kq hold one row.  Past the end of a
 // row its last octet is read again, taken out by value in `operand`.
@@ -83,7 +91,9 @@ struct RowValues {
     }
 };
 
-template <int KS, int RT, int NW>  // k-steps of 32 coordinates, row tiles of 16 per wave, computing waves
+// KS k-steps of 32 coordinates, NW multiplying waves.  The waves per SIMD asked for are those of two workgroups on a CU, of
+// one above 256 columns, where its tiles fill more than half of the shared memory.
+template <int KS, int NW>
 __global__ __launch_bounds__(64 * NW + 128, NW == 8 ? 5 : KS <= 8 ? 3 : 2) void grouped_score_kernel(ScoreArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ uint4 tile[2][2 * KS * 2 * 64];  // [buffer][(column tile, k-step, part, lane)]
@@ -140,33 +150,29 @@ __global__ __launch_bounds__(64 * NW + 128, NW == 8 ? 5 : KS <= 8 ? 3 : 2) void 
         return;
     }
 
-    // ---- enrol side: a[i][s][part] = coordinates 32 s + 8 kq .. + 7 of row i0 + 16 i + r16
-    const int64_t i0 = (i_blk * NW + wave) * (16 * RT);
+    // ---- enrol side: a[s][part] = coordinates 32 s + 8 kq .. + 7 of row i0 + r16
+    const int64_t i0 = (i_blk * NW + wave) * 16;
     const bool live = i0 < n1;  // this wave has rows
-    f16x8 a[RT][KS][2];
-    int rs[RT];
-    // result rows of this lane; a row past the end holds the last row's scores (its operand is a copy) and stores
+    f16x8 a[KS][2];
+    int rs = 0;
+    // result row of this lane; a row past the end holds the last row's scores (its operand is a copy) and stores
     // them to the same place, so that no store depends on a comparison
-    float* dst[RT];
+    float* dst = nullptr;
     if (live) {
+        int64_t row = i0 + r16;
+        row = row < n1 ? row : n1 - 1;
+        dst = g.S + g.blocks[e] + row * n2 + j_beg + 4 * kq;
+        RowValues<KS> v;
+        v.fetch(g.G1 + (g.off1[e] + row) * g.ld1, g.kp, kq);
+        rs = v.scale();
+        const float f = exp2_int(rs);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            int64_t row = i0 + 16 * i + r16;
-            row = row < n1 ? row : n1 - 1;
-            dst[i] = g.S + g.blocks[e] + row * n2 + j_beg + 4 * kq;
-            RowValues<KS> v;
-            v.fetch(g.G1 + (g.off1[e] + row) * g.ld1, g.kp, kq);
-            rs[i] = v.scale();
-            const float f = exp2_int(rs[i]);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) v.operand(s, f, g.kp, kq, a[i][s][0], a[i][s][1]);
-        }
+        for (int s = 0; s < KS; ++s) v.operand(s, f, g.kp, kq, a[s][0], a[s][1]);
     }
     auto multiply = [&](int it, bool whole) {
         const int buf = it & 1;
-        f32x4 acc[RT][2];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        f32x4 acc[2];
+        acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
         f16x8 b[2][2][2];  // [k-step parity][column tile][part]
         auto request = [&](int s) {
 #pragma unroll
@@ -183,28 +189,22 @@ __global__ __launch_bounds__(64 * NW + 128, NW == 8 ? 5 : KS <= 8 ? 3 : 2) void 
             for (int p = 0; p < 3; ++p)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-                        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[s & 1][c][p == 0], a[i][s][p == 1],
-                                                                           acc[i][c], 0, 0, 0);
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[s & 1][c][p == 0], a[s][p == 1], acc[c], 0, 0, 0);
         }
-        // lane: columns 32 it + 16 c + 4 kq .. + 3 of enrol row i0 + 16 i + r16
+        // lane: columns 32 it + 16 c + 4 kq .. + 3 of enrol row i0 + r16
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int j = 32 * it + 16 * c;
             const int4 cs = *reinterpret_cast<const int4*>(&scale[buf][16 * c + 4 * kq]);
+            // one shift by the sum of both exponents: neither scale alone may leave the range
+            const f32x4 r = {ldexpf(acc[c][0], -rs - cs.x), ldexpf(acc[c][1], -rs - cs.y),
+                             ldexpf(acc[c][2], -rs - cs.z), ldexpf(acc[c][3], -rs - cs.w)};
+            if (whole) {
+                *reinterpret_cast<f32x4_a4*>(dst + j) = r;
+            } else {
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                // one shift by the sum of both exponents: neither scale alone may leave the range
-                const f32x4 r = {ldexpf(acc[i][c][0], -rs[i] - cs.x), ldexpf(acc[i][c][1], -rs[i] - cs.y),
-                                 ldexpf(acc[i][c][2], -rs[i] - cs.z), ldexpf(acc[i][c][3], -rs[i] - cs.w)};
-                if (whole) {
-                    *reinterpret_cast<f32x4_a4*>(dst[i] + j) = r;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (j + 4 * kq + q < ncol) dst[i][j + q] = r[q];
-                }
+                for (int q = 0; q < 4; ++q)
+                    if (j + 4 * kq + q < ncol) dst[j + q] = r[q];
             }
         }
     };
@@ -223,10 +223,10 @@ __global__ __launch_bounds__(64 * NW + 128, NW == 8 ? 5 : KS <= 8 ? 3 : 2) void 
 
 template <int KS>
 int launch_score(const ScoreArgs& g, hipStream_t stream) {
-    constexpr int RT = KS == 6 ? 2 : 1, NW = KS <= 5 ? 8 : 4;
+    constexpr int NW = score_waves(KS);
     const int64_t grid = xcd_grid(g.n_tasks, SCORE_RUN);
     HYPMI_REQUIRE(fits_launch(grid, 64 * NW + 128), "grouped_score: too many workgroups");
-    hipLaunchKernelGGL((grouped_score_kernel<KS, RT, NW>), dim3((unsigned)grid), dim3(64 * NW + 128), 0, stream, g);
+    hipLaunchKernelGGL((grouped_score_kernel<KS, NW>), dim3((unsigned)grid), dim3(64 * NW + 128), 0, stream, g);
     HYPMI_HIP(hipGetLastError());
     return HYPMI_OK;
 }
@@ -237,7 +237,7 @@ using namespace hypmi_detail;
 
 extern "C" int hypmi_grouped_score_rows(int kp) {
     if (kp <= 0 || kp % 8 != 0 || kp > 512) return 0;
-    return (kp + 31) / 32 <= 6 ? 128 : 64;
+    return 16 * score_waves((kp + 31) / 32);
 }
 
 extern "C" int hypmi_grouped_score_span(void) { return SCORE_SPAN; }
