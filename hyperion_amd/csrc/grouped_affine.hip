@@ -219,7 +219,8 @@ __global__ __launch_bounds__(512, RT == 1 ? 1 : 4) void grouped_affine_kernel(Af
     // the chunk loop of a wave with `tiles` column tiles
     auto walk = [&](auto tiles_tag) {
         constexpr int N = decltype(tiles_tag)::value;
-        // k-steps of weights in registers; 4 and 8 with tiles of 16 take 9.7 and 10.3 us for the twelve rows above, 2 takes 9.0
+        // k-steps of weights in registers: 2, 4 and 8 with tiles of 16 take 9.0, 9.7 and 10.3 us for the twelve rows above, 1
+        // and 2 with tiles of 64 20.7 and 16.9 us for 40 rows a group of 512 -> 77, 20.6 and 20.4 for 128 of 200 -> 200
         constexpr int WS = RT == 8 ? 1 : 2;
         const uint4* w0p = wp + ((int64_t)e * g.ct + ct0) * w_tile;
         const uint4* w1p = wp + ((int64_t)e * g.ct + ct1) * w_tile;

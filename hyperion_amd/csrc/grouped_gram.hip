@@ -16,12 +16,14 @@
 // chunks of one length; every chunk writes its block to a slot of the workspace and a second kernel adds the slots in
 // chunk order.  No sum depends on scheduling.
 //
-// Measured: 57 300 float64 rows of 7 groups, d = 512, 299 us back to back, 14 of them the second kernel (50 TFLOP/s);
-// 25 600 fp32 rows of 200 groups, d = 200, 48 us, of which the matrix instructions are 20 and the writing of 64 MB 13.
+// Measured: 57 300 float64 rows of 7 groups, d = 512, 317 us back to back, 14 of them the second kernel (47.5 TFLOP/s);
+// 25 600 fp32 rows of 200 groups, d = 200, 45 us, of which the matrix instructions are 20 and the writing of 64 MB 13.
 // GRAM_SPLIT: with 200 groups of 96 rows a wave per block takes 32 us and four waves 44, with 384 and more rows 47 to
 // 60 and 50 to 48; the ragged groups above take 50.3 / 48.9 / 49.9 / 51.6 / 53.2 us with a limit of 128 / 192 / 256 /
-// 320 / 400 rows.  GRAM_SPAN of 1024 / 1536 / 2048 / 4096 rows: 316 / 312 / 299 / 324 us of the first
-// case (345 with 4096 and chunks that are full but for the last).
+// 320 / 400 rows.  GRAM_SPAN of 1024 / 1536 / 2048 / 4096 rows, the mean of three sets of sizes in us: float64, d = 512, 7
+// groups 336 / 331 / 329 / 331; d = 200, 3 groups 136 / 133 / 137 / 148; fp32, d = 200, 7 groups 78 / 77 / 76 / 88;
+// d = 150, 20 groups 56 / 57 / 60 / 69; one group of 30 000 rows, d = 128, 43 / 33 / 35 / 47.  From 1536 to 2048 the sizes
+// of the groups decide, 4096 leaves too few chunks, 1024 adds a slot per chunk to write and read again.
 #include "grouped.h"
 
 #include <type_traits>
