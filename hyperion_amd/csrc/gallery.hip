@@ -18,7 +18,8 @@
 // nibble above it), and one packed fp16 operation makes c - 8 of either, exactly.  (Left as the sub-normal number
 // that the bare nibble is, without that operation, a code is multiplied exactly but added with ten bits less:
 // 3e-6 of the sum of magnitudes instead of 1e-7, measured.)  Test rows are scaled by a power of two and held as
-// fp16 pairs (see score_split.hip), so a score is the fp32-accurate product of the row that the codes stand for.
+// fp16 pairs (see score_split.hip), so a score is the product with the row that the codes stand for, the
+// coordinates of the test to 22 bits or to 2^-39 of its largest.
 // The contraction of one instruction is one scale group: its result is multiplied by the scale and added up in
 // fp32.
 //

@@ -3,8 +3,8 @@ of a trial set, the partitions of a gallery), each group with its own matrix, it
 block of scores, in one launch.  The names here are part of hyperion_amd.engine.
 
 A batch is described once, by a RowGroups (sizes on the host, tables on the device) and, for products of
-two sides, a GroupPairs; the operators themselves neither wait for the device nor send it anything, so they
-can be captured in a HIP graph.  Inputs have to be on one device; the work runs on that device's current
+two sides, a GroupPairs; on device tensors the operators themselves neither wait for the device nor send it anything,
+so they can be captured in a HIP graph.  Inputs have to be on one device; the work runs on that device's current
 stream.  A RowGroups, a GroupPairs and an AffineBank are complete when they have been made (which waits for the
 current stream) and can be used on any stream at once; a Q4Rows is filled by a launch on the stream it is made on, for
 which another stream waits as for any tensor."""
@@ -375,7 +375,7 @@ def _packed(G, groups, what):
 
 def grouped_pack(s, groups, maps, c, sides="both"):
     """Packed rows of the projected rows s [n, K] (device fp32, in group order) by the maps of their group: maps
-    [E, 4, K] = shift_t, scale_t, shift_n, scale_n, c [E] (host or device).  Returns (enrol-side, test-side) rows
+    [E, 4, K] = shift_t, scale_t, shift_n, scale_n, c [E] (host arrays are sent, which waits).  Returns (enrol-side, test-side) rows
     [n, kp]; sides "enrol" or "test": the other is None."""
     torch = _torch()
     s, ld = _device_rows(s, _kinds("rows"), "s")
@@ -406,7 +406,8 @@ def grouped_score_supported(kp):
 
 def grouped_score(G1, G2, pairs, out=None):
     """Scores of packed enrol rows against packed test rows of the same group (Plan.prologue, both [n, kp]):
-    the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e)."""
+    the flat device fp32 result of `pairs` (pairs.block(flat, e) is the [n1, n2] block of group e).  An element of a
+    row counts to 22 bits, or to 2^-39 of the largest magnitude of its row where that is more, as in score."""
     same = G2 is G1 and pairs.cols is pairs.rows  # self-scores: checked once
     G1, ld1 = _packed(G1, pairs.rows, "G1")
     G2, ld2 = (G1, ld1) if same else _packed(G2, pairs.cols, "G2")

@@ -573,7 +573,8 @@ int hypmi_grouped_pack(const float* s, int64_t lds, int K, const int64_t* offset
 /* S_e = G1_e G2_e^T for every group e from packed rows (hypmi_prologue; widths up to 512, multiples of 8; rows
  * 16-byte aligned): n1_e x n2_e scores, row-major without padding, at element block_offsets[e] of S.  tasks:
  * prefix sums of ceil(n1_e / hypmi_grouped_score_rows(kp)) * ceil(n2_e / hypmi_grouped_score_span()).
- * hypmi_grouped_score_rows returns 0 for a width without a kernel.  Accuracy as hypmi_score_pair. */
+ * hypmi_grouped_score_rows returns 0 for a width without a kernel.  Accuracy as hypmi_score_pair: an element of either
+ * row counts to 22 bits, or to 2^-39 of the largest magnitude of its row where that is more; sums are fp32. */
 int hypmi_grouped_score_rows(int kp);
 int hypmi_grouped_score_span(void);
 int hypmi_grouped_score(const float* G1, int64_t ld1, const float* G2, int64_t ld2, int kp, const int64_t* offsets1,
@@ -610,8 +611,9 @@ int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* offsets, co
                   int64_t n_blocks, void* codes, void* scales, float* q, void* stream);
 
 /* Scores of test-side packed rows [g, 1, q + c] against the gallery, group by group: S_e [tests_e x rows_e],
- * row-major without padding, at element out_offsets[e] of S; each is the fp32-accurate product with the row that
- * the codes stand for (hyperion/pdfs/plda/splda.py:312-315).  offsets_t delimits the tests, offsets_g the gallery
+ * row-major without padding, at element out_offsets[e] of S; each is the product with the row that the codes stand
+ * for (hyperion/pdfs/plda/splda.py:312-315), the coordinates of a test counting to 22 bits, or to 2^-39 of the largest
+ * magnitude of their row where that is more, sums in fp32.  offsets_t delimits the tests, offsets_g the gallery
  * rows.  G: 16-byte aligned rows, ldg a multiple of 4, at least k + 2 and at least k rounded up to 8 readable.
  * tasks: prefix sums of ceil(rows_e / task_rows) * ceil(tests_e / task_tests), task_tests 16, 32 or 64, task_rows
  * any multiple of 64. */
