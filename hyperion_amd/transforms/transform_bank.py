@@ -1,10 +1,13 @@
 """Pre-processing chains by group: every row goes through the chain of its domain, condition or recording."""
+import copy
+
 import numpy as np
 
 from .. import engine
 from ..fold import fold_chain
 from ..hyp_defs import float_cpu
 from ..hyp_model import HypModel
+from .transform_list import TransformList
 
 
 class TransformBank(HypModel):
@@ -80,3 +83,29 @@ class TransformBank(HypModel):
             ids._check(y, "x")
             y = y.to(torch.float32, copy=True)
         return y if is_dev else engine.to_host(y, float_cpu())
+
+    # ---- model files: the transforms of chain e under <name>/<e>/<i>, as a TransformList keeps its own ----------
+    def _stored(self):
+        prefix = "" if self.name is None else self.name + "/"
+        chains = []
+        for e, chain in enumerate(self.chains):
+            chains.append([copy.copy(t) for t in chain])
+            for i, t in enumerate(chains[-1]):
+                t.name = "%s%d/%d" % (prefix, e, i)
+        return chains
+
+    def save_params(self, f):
+        for chain in self._stored():
+            for t in chain:
+                t.save_params(f)
+
+    @classmethod
+    def load_params(cls, f, config):
+        chains = config["chains"]
+        return cls([TransformList.load_params(f, {"name": None, "transforms": chains[str(e)]}).transforms
+                    for e in range(len(chains))], name=config["name"])
+
+    def get_config(self):
+        config = super().get_config()
+        config["chains"] = {e: {i: t.get_config() for i, t in enumerate(c)} for e, c in enumerate(self._stored())}
+        return config
