@@ -17,7 +17,7 @@
 // for the kernel alone, nothing for passes that follow one another).  Test rows
 // are the first operand of the matrix instruction, so a lane ends up with four neighbouring scores of one enrol row.
 //
-// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 33 to 40 us by the box, 12
+// Measured at a packed width of 152: 200 recordings of 12 to 900 segments (16.2 M scores) 33 to 40 us from card to card, 12
 // domains of 300 to 20000 test vectors (68.9 M scores) 136, of which the kernel alone 107 to 126 after a pause: 2.0 TB/s
 // of results.  The domains write 334 MB for 276 (a row of a block starts anywhere in a line) and read 91 MB for 20;
 // without the stores they take 95 us, with the stores and one multiplication per span 76 to 85, so neither alone is the
@@ -46,8 +46,8 @@ struct ScoreArgs {
 constexpr int SCORE_RUN = 8;     // tasks dealt to an XCD at a time
 constexpr int SCORE_SPAN = 512;  // test rows one workgroup walks at most
 
-// Multiplying waves of a workgroup, 16 enrol rows each.  Recordings (17.5 M scores) / domains (12.5 M) with eight waves, with
-// four, with four that take 32 rows each, in us: 3 k-steps 35 / 23, 39 / 27, 35 / 24; 5 k-steps 40 / 26, 46 / 30,
+// Multiplying waves of a workgroup, 16 enrol rows each.  Recordings (17.5 M scores) / domains (12.5 M) with eight
+// waves, with four, with four that take 32 rows each, in us: 3 k-steps 35 / 23, 39 / 27, 35 / 24; 5 k-steps 40 / 26, 46 / 30,
 // 40 / 27; 6 k-steps 53 / 32, 63 / 39, 62 / 34.  Eight would be faster above 192 columns too (8 k-steps 74 / 39 against
 // 85 / 56, 16 k-steps 144 / 72 against 160 / 103), where callers count their tasks in 64 rows.
 constexpr int score_waves(int ksteps) { return ksteps <= 6 ? 8 : 4; }

@@ -122,3 +122,17 @@ def test_a_gallery_of_512_latent_dimensions():
     want = plda.llr_1vs1(x[::2], x[1::2])
     got = PLDAGallery(plda).enrol(x[::2]).llr(x[1::2])
     assert np.std(got - want) <= 0.2 * np.std(want)
+
+
+def test_empty_galleries_and_partitions():
+    import numpy as np
+
+    g = _gallery(5)
+    x = np.random.RandomState(2).randn(6, 24)
+    assert g.enrol(x[:0]).llr(x).shape == (0, 6)
+    rows, best = g.identify(x, 3)
+    assert (rows == -1).all() and np.isneginf(best).all()
+    g.enrol(x, [2, 2, 0, 2, 0, 2], 4)
+    rows, best = g.identify(x, 3, [1, 3, 0, 2, 2, 1])
+    assert (rows[[0, 1, 5]] == -1).all() and set(rows[2]) == {2, 4, -1} and set(rows[3]) | set(rows[4]) <= {0, 1, 3, 5}
+    assert [s.shape for _, _, s in g.llr(x, [1, 3, 0, 2, 2, 1])] == [(2, 1), (0, 2), (4, 2), (0, 1)]
