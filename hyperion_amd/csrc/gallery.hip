@@ -330,7 +330,7 @@ extern "C" int hypmi_q4_rows(const float* G, int64_t ldg, int k, const int64_t* 
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     const int ks = q4_ksteps(k);
     HYPMI_REQUIRE(ks > 0, "q4_rows: %d coordinates (1 to 512)", k);
-    HYPMI_REQUIRE(n_groups >= 0 && n_blocks >= 0 && ldg >= k + 1, "q4_rows: bad shape");
+    HYPMI_REQUIRE(fits_groups(n_groups) && n_blocks >= 0 && ldg >= k + 1, "q4_rows: bad shape");
     if (n_blocks == 0) return HYPMI_OK;
     HYPMI_REQUIRE(G && offsets && blocks && codes && scales && q, "q4_rows: null pointer");
     HYPMI_REQUIRE(aligned16(codes) && aligned16(scales), "q4_rows: buffers must be 16-byte aligned");
@@ -351,7 +351,7 @@ extern "C" int hypmi_q4_score(const void* codes, const void* scales, const float
     HYPMI_REQUIRE(ks > 0, "q4_score: %d coordinates (1 to 512)", k);
     HYPMI_REQUIRE(task_tests == 16 || task_tests == 32 || task_tests == 64, "q4_score: 16, 32 or 64 tests per task");
     HYPMI_REQUIRE(task_rows > 0 && task_rows % Q4_BLOCK == 0, "q4_score: task_rows must be a multiple of 64");
-    HYPMI_REQUIRE(n_groups >= 0 && n_tasks >= 0, "q4_score: bad shape");
+    HYPMI_REQUIRE(fits_groups(n_groups) && n_tasks >= 0, "q4_score: bad shape");
     HYPMI_REQUIRE(ldg % 4 == 0 && ldg >= k + 2 && ldg >= (k + 7) / 8 * 8, "q4_score: bad leading dimension");
     if (n_tasks == 0) return HYPMI_OK;
     HYPMI_REQUIRE(codes && scales && q && G && offsets_t && offsets_g && blocks && out_offsets && tasks && S,

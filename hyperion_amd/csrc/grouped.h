@@ -36,6 +36,9 @@ __device__ __forceinline__ int64_t xcd_task(int64_t b, int64_t n, int run) {
     return t < n ? t : -1;
 }
 
+// What find_group counts in 32 bits: the number of groups, and that and a step more.
+inline bool fits_groups(int n) { return n >= 0 && n <= 1 << 30; }
+
 // A launch holds fewer than 2^32 work-items in a dimension.
 inline bool fits_launch(int64_t blocks, int threads) { return blocks >= 0 && blocks <= 0xffffffffLL / threads; }
 

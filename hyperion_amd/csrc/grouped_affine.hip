@@ -561,7 +561,7 @@ extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int 
                                     const int32_t* dims, int d_out, int lnorm, float* y, int64_t ldy, int cols_y,
                                     void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    HYPMI_REQUIRE(n_groups >= 0 && n_rows >= 0 && n_tiles >= 0 && d_in > 0 && d_out > 0, "grouped_affine: bad shape");
+    HYPMI_REQUIRE(fits_groups(n_groups) && n_rows >= 0 && n_tiles >= 0 && d_in > 0 && d_out > 0, "grouped_affine: bad shape");
     HYPMI_REQUIRE(n_rows <= 0x7fffffffLL, "grouped_affine: at most 2^31 - 1 rows");
     HYPMI_REQUIRE(x_type >= HYPMI_F32 && x_type <= HYPMI_BF16, "grouped_affine: vectors must be fp32, fp16 or bf16");
     HYPMI_REQUIRE(tile_rows == 16 || tile_rows == 64 || tile_rows == 128, "grouped_affine: tiles of 16, 64 or 128 rows");
@@ -591,7 +591,7 @@ extern "C" int hypmi_grouped_affine(const void* x, int x_type, int64_t ldx, int 
 extern "C" int hypmi_grouped_pack(const float* s, int64_t lds, int K, const int64_t* offsets, int n_groups, int64_t n_rows,
                                   const float* maps, const float* c, float* G1, float* G2, int kp, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    HYPMI_REQUIRE(K > 0 && kp >= K + 2 && lds >= K && n_groups >= 0 && n_rows >= 0, "grouped_pack: bad shape");
+    HYPMI_REQUIRE(K > 0 && kp >= K + 2 && lds >= K && fits_groups(n_groups) && n_rows >= 0, "grouped_pack: bad shape");
     HYPMI_REQUIRE(G1 || G2, "grouped_pack: no result asked for");
     if (n_rows == 0) return HYPMI_OK;
     HYPMI_REQUIRE(s && offsets && maps && c, "grouped_pack: null pointer");

@@ -311,7 +311,7 @@ extern "C" int hypmi_grouped_gram_f64(const void* x, int x_type, int64_t ldx, in
                                       int n_groups, int64_t n_units, int64_t n_slots, const int32_t* order, double* C,
                                       double* F, void* workspace, int64_t workspace_bytes, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    HYPMI_REQUIRE(n_groups >= 0 && n_units >= 0 && n_slots >= 0 && d > 0, "grouped_gram: bad shape");
+    HYPMI_REQUIRE(fits_groups(n_groups) && n_units >= 0 && n_slots >= 0 && d > 0, "grouped_gram: bad shape");
     HYPMI_REQUIRE(x_type == HYPMI_F32 || x_type == HYPMI_F64, "grouped_gram: vectors must be fp32 or fp64");
     HYPMI_REQUIRE(ldx >= d, "grouped_gram: bad leading dimension");
     if (n_groups == 0) return HYPMI_OK;

@@ -246,7 +246,7 @@ extern "C" int hypmi_grouped_score(const float* G1, int64_t ld1, const float* G2
                                    const int64_t* offsets1, const int64_t* offsets2, const int64_t* block_offsets,
                                    const int64_t* tasks, int n_groups, int64_t n_tasks, float* S, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    HYPMI_REQUIRE(n_groups >= 0 && n_tasks >= 0, "grouped_score: bad shape");
+    HYPMI_REQUIRE(fits_groups(n_groups) && n_tasks >= 0, "grouped_score: bad shape");
     HYPMI_REQUIRE(hypmi_grouped_score_rows(kp) > 0, "grouped_score: packed width %d (a multiple of 8 up to 512)", kp);
     HYPMI_REQUIRE(ld1 >= kp && ld2 >= kp && ld1 % 4 == 0 && ld2 % 4 == 0, "grouped_score: bad leading dimension");
     if (n_tasks == 0) return HYPMI_OK;

@@ -92,11 +92,11 @@ class RowGroups(_Plan):
         sizes = np.asarray(sizes)
         if sizes.ndim != 1 or (sizes.size and sizes.dtype.kind not in "iu"):
             raise ValueError("group sizes must be a 1-D sequence of integers")
+        if sizes.size > 1 << 30:  # the search for a row's group counts in 32 bits, with some steps to spare
+            raise ValueError("at most 2^30 groups")
         sizes = sizes.astype(np.int64)
         if sizes.size and sizes.min() < 0:
             raise ValueError("group sizes must not be negative")
-        if sizes.size > 0x7fffffff:
-            raise ValueError("at most 2^31 - 1 groups")
         if sizes.sum(dtype=np.float64) > 2.0 ** 40:
             raise ValueError("at most 2^40 rows")
         self.sizes = sizes

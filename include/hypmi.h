@@ -526,8 +526,8 @@ int hypmi_score_extract(const float* S, int64_t lds, int64_t ne, int64_t nt, con
 
 /* ---- grouped operators: rows that fall into groups of unequal sizes ----------------------------- */
 
-/* The rows of group e are offsets[e] .. offsets[e + 1] - 1 (int64, device, n_groups + 1 entries, ascending
- * from 0; groups may be empty), or, where a call takes `order`, the rows order[offsets[e]] ..
+/* The rows of group e are offsets[e] .. offsets[e + 1] - 1 (int64, device, n_groups + 1 entries, at most 2^30
+ * groups, ascending from 0; groups may be empty), or, where a call takes `order`, the rows order[offsets[e]] ..
  * order[offsets[e + 1] - 1].  Work is cut into tiles that never cross a group; a call that is cut takes the
  * prefix sums of its tile counts (int64, device, n_groups + 1 entries from 0) and their total, which is the
  * size of the launch, so that neither the host nor the device has to wait for the other.  The tables are not
